@@ -70,16 +70,14 @@ def weight_bytes_per_step(model) -> int:
 def kv_bytes_per_token(model) -> int:
     """Bytes of keys and values one cached token takes over all layers."""
     kv, _, source = model.cache_needs()
-    width = torch.empty((), dtype=model.dtype).element_size()
-    return sum(need.kv_heads * (need.head_dim + need.v_dim) * width for need, src in zip(kv, source) if need is not None and src is None)
+    return sum(need.token_bytes(model.dtype) for need, src in zip(kv, source) if need is not None and src is None)
 
 
 def kv_read_bytes_per_token(model) -> int:
     """Bytes of keys and values a decode step reads per cached token: every run that attends reads
     them, also one that reads another run's cache."""
     kv, _, _ = model.cache_needs()
-    width = torch.empty((), dtype=model.dtype).element_size()
-    return sum(need.kv_heads * (need.head_dim + need.v_dim) * width for need in kv if need is not None)
+    return sum(need.token_bytes(model.dtype) for need in kv if need is not None)
 
 
 def kv_read_bytes(model, context: float) -> float:
@@ -87,7 +85,6 @@ def kv_read_bytes(model, context: float) -> float:
     reads only the window's tokens, one with chunks its chunk's, a coarser cache (a mixer's summary) one entry for each of
     its blocks."""
     kv, _, _ = model.cache_needs()
-    width = torch.empty((), dtype=model.dtype).element_size()
     chunked = {}                    # a run whose mask is chunks reads fewer keys than its cache keeps
     for index, run in enumerate(model.spec.schedule):
         for user, mixer in zip(model.users[index], model.layers[run.layer].mixers()):
@@ -97,7 +94,7 @@ def kv_read_bytes(model, context: float) -> float:
         held = context / need.every
         return held if need.window is None else min(held, need.window)
 
-    return sum(need.kv_heads * (need.head_dim + need.v_dim) * width * chunked.get(user, entries(need)) for user, need in enumerate(kv) if need is not None)
+    return sum(need.token_bytes(model.dtype) * chunked.get(user, entries(need)) for user, need in enumerate(kv) if need is not None)
 
 
 def state_bytes_per_sequence(model) -> int:

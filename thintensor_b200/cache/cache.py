@@ -4,7 +4,7 @@ of the schedule that keeps any, and per-sequence state of fixed size.
 Runs with the same need (kv heads, head size, window) form a *group* with storage of
 its own: per run one piece of memory that holds the key pool (``[blocks, kv_heads, block_tokens, head_dim]``)
 followed by the value pool (transposed inside a block, ``[blocks, kv_heads, value_dim, block_tokens]``; a value
-head may have another size than a key head), and one block table, so that, say, windowed layers give blocks back
+head may have another size than a key head; a group in 4 bits holds both as bytes, ``[blocks, kv_heads, bytes]``), and one block table, so that, say, windowed layers give blocks back
 while full-attention layers keep theirs.  State needs are grouped the same way into
 ``[runs, slots, *shape]`` tensors, zeroed when a slot is handed out.
 
@@ -30,7 +30,7 @@ class KVGroup:
     need: KVNeed
     runs: list[int]                 # schedule entries that own a cache in this group
     table: BlockTable
-    storage: torch.Tensor | None    # [runs, blocks * kv_heads * BLOCK_TOKENS * (head_dim + value_dim)]: keys, then values
+    storage: torch.Tensor | None    # [runs, blocks * kv_heads * BLOCK_TOKENS * (head_dim + value_dim)]: keys, then values; in 4 bits: their bytes
     num_blocks: int = 0             # blocks of this group's pool
 
     def bytes(self) -> int:
@@ -49,8 +49,8 @@ class RunCache:
     """What one run of the schedule sees of the cache."""
 
     group: int | None               # index of its KV group, None if it keeps no keys
-    k_pool: torch.Tensor | None     # [blocks, kv_heads, BLOCK_TOKENS, head_dim]
-    v_pool: torch.Tensor | None     # [blocks, kv_heads, value_dim, BLOCK_TOKENS]
+    k_pool: torch.Tensor | None     # [blocks, kv_heads, BLOCK_TOKENS, head_dim]; in 4 bits: uint8 [blocks, kv_heads, bytes]
+    v_pool: torch.Tensor | None     # [blocks, kv_heads, value_dim, BLOCK_TOKENS]; likewise
     writes: bool                    # False when the run reads another run's cache
     window: int | None
     summary: "RunCache | None" = None   # the mixer's coarser cache (one entry for several tokens), where it keeps one
@@ -102,7 +102,7 @@ class SequenceCache:
             if kv_needs[run] is None or kv_needs[source] is None:
                 raise CacheError(f"run {run} reads the cache of run {source}, but one of them keeps no keys")
             a, b = kv_needs[run], kv_needs[source]
-            if (a.kv_heads, a.head_dim, a.v_dim, a.every) != (b.kv_heads, b.head_dim, b.v_dim, b.every):
+            if (a.kv_heads, a.head_dim, a.v_dim, a.every, a.bits) != (b.kv_heads, b.head_dim, b.v_dim, b.every, b.bits):
                 raise CacheError(f"run {run} reads the cache of run {source}, whose key/value shape differs")
             if b.window is not None and (a.window is None or a.window > b.window):
                 # the source's group gives blocks back by the source's window; a reader that looks
@@ -127,6 +127,10 @@ class SequenceCache:
             for group in self.kv_groups:
                 per_block = group.need.kv_heads * BLOCK_TOKENS
                 shape = (len(group.runs), group.num_blocks * per_block * (group.need.head_dim + group.need.v_dim))
+                if group.need.bits == 4:            # bytes; a block that nothing was written to reads as zeros
+                    shape = (len(group.runs), group.num_blocks * BLOCK_TOKENS * group.need.token_bytes(dtype))
+                    group.storage = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+                    continue
                 # zeros, not empty: a tensor-core product multiplies the unused tail of a block by a
                 # probability of exactly zero, which must not meet a NaN left in fresh memory
                 group.storage = torch.zeros(shape, dtype=dtype, device=self.device)
@@ -199,6 +203,10 @@ class SequenceCache:
         k = v = None
         if g.storage is not None:
             need = g.need
+            if need.bits == 4:
+                half = g.storage.shape[1] // 2
+                k, v = (part.view(g.num_blocks, need.kv_heads, -1) for part in (g.storage[index, :half], g.storage[index, half:]))
+                return RunCache(group, k, v, self._cache_from[run] is None, need.window)
             keys = g.num_blocks * need.kv_heads * BLOCK_TOKENS * need.head_dim
             k = g.storage[index, :keys].view(g.num_blocks, need.kv_heads, BLOCK_TOKENS, need.head_dim)
             v = g.storage[index, keys:].view(g.num_blocks, need.kv_heads, need.v_dim, BLOCK_TOKENS)

@@ -31,10 +31,14 @@ def _build(role_registry, spec: PartSpec) -> BuiltPart:
 
 
 class DecoderModel:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device | str | None):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device | str | None, cache_bits: int | None = None):
+        """``cache_bits`` 4: keys and values are kept in 4 bits (every mixer that keeps any must be able to); None: in ``dtype``."""
         spec.validate()
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"the engine runs in float32 or bfloat16, not {dtype}")
+        if cache_bits not in (None, 4):
+            raise ValueError(f"keys and values are kept in the engine's type (None) or in 4 bits, not {cache_bits!r}")
+        self.cache_bits = cache_bits
         self.spec = spec
         self.dtype = dtype
         self.device = torch.device(device) if device is not None else None
@@ -59,6 +63,12 @@ class DecoderModel:
                 raise ValueError(f"arrangement {layer.arrangement!r} has no role {sorted(unknown)[0]!r}")
             self._layer_parts.append(built)
             self.layers.append(arrangement_cls({role: b.part for role, b in built.items()}, **dict(layer.params)))
+        if cache_bits == 4:
+            for number, layer in enumerate(self.layers):
+                for mixer in layer.mixers():
+                    reason = mixer.no_4bit_cache(dtype) if mixer.cache_need() is not None else None
+                    if reason is not None:
+                        raise ValueError(f"layer {number} cannot keep its cache in 4 bits: {reason}")
         self.bound = False
         self.device_driven = False
         self.cache_needs()          # sets self.users
@@ -118,6 +128,8 @@ class DecoderModel:
                 raise ValueError(f"a run of layer {run.layer} reads the cache of a run with another number of mixers")
             for i, mixer in enumerate(mixers):
                 need = mixer.cache_need()
+                if need is not None and self.cache_bits is not None:
+                    need = replace(need, bits=self.cache_bits)
                 kv.append(need)
                 state.append(list(mixer.state_needs()))
                 # only keys are shared: a mixer without keys has nothing to read there, and states are always a run's own

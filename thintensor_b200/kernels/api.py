@@ -1238,6 +1238,135 @@ def weighted_pair(a: torch.Tensor, wa: float, b: torch.Tensor, wb: float, out: t
     _check(fn(_ptr(a), a.shape[0], a.stride(0), wa, _ptr(b), b.shape[0], b.stride(0), wb, _ptr(out), out.numel(), _stream()), "weighted_pair")
 
 
+# ------------------------------------------------------------------------ cache in 4 bits
+CACHE_4BIT_DIMS = (32, 64, 96, 128)
+
+
+def cache_4bit_supports(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int) -> bool:
+    """Whether keys and values can be held in 4 bits: bfloat16 activations, head size 32, 64, 96 or 128, at most 16 query heads
+    per key/value head."""
+    return dtype == torch.bfloat16 and head_dim in CACHE_4BIT_DIMS and kv_heads > 0 and heads % kv_heads == 0 and 1 <= heads // kv_heads <= 16
+
+
+def cache_4bit_bytes(head_dim: int) -> int:
+    """Bytes of one head's keys (or values) in one block of 64 tokens: 4 bits a number and two bfloat16 numbers for each 32."""
+    return BLOCK_TOKENS * (head_dim // 2 + head_dim // 32 * 4)
+
+
+def _check_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
+                kv_heads: int, head_dim: int, status: torch.Tensor) -> None:
+    for t, name in ((k_pool, "the 4-bit key pool"), (v_pool, "the 4-bit value pool")):
+        _need(t, torch.uint8, name)
+        if t.dim() != 3 or tuple(t.shape[1:]) != (kv_heads, cache_4bit_bytes(head_dim)):
+            raise KernelError(f"{name} must be [blocks, {kv_heads}, {cache_4bit_bytes(head_dim)}] bytes, got {tuple(t.shape)}")
+        _need_aligned(t, name)
+    if k_pool.shape[0] != v_pool.shape[0]:
+        raise KernelError("the 4-bit pools must have as many blocks of values as of keys")
+    _check_step(table, cu, len_before, sequences, status)
+
+
+def _check_step(table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int, status: torch.Tensor) -> None:
+    for t, name in ((table, "the block table"), (cu, "token offsets"), (len_before, "lengths"), (status, "the status word")):
+        _need(t, torch.int32, name)
+    if sequences < 1 or table.dim() != 2 or table.shape[0] < sequences or cu.numel() < sequences + 1 or len_before.numel() < sequences:
+        raise KernelError(f"a step of {sequences} sequences needs a table row and a length for each and one offset more, got "
+                          f"{tuple(table.shape)}, {len_before.numel()}, {cu.numel()}")
+
+
+def rope_append_4bit(qkv: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int, attention_scaling: float, q_out: torch.Tensor,
+                     k_pool: torch.Tensor | None, v_pool: torch.Tensor | None, table: torch.Tensor, cu: torch.Tensor,
+                     len_before: torch.Tensor, sequences: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int,
+                     status: torch.Tensor, interleaved: bool = False) -> None:
+    """:func:`rope_append` for a cache in 4 bits: q and k of the float32 partial sums ``qkv`` [splits, tokens, cols] are rotated on their first
+    ``rotary_dim`` numbers (halves, or neighbouring pairs with ``interleaved``; the angle is formed in float64), q goes to ``q_out``
+    (bfloat16 [tokens, heads * head_dim]), k and v are brought to 4 bits, a scale and a least value for each 32 numbers of a head, and put into their places
+    of ``k_pool`` / ``v_pool`` (uint8 ``[blocks, kv_heads, cache_4bit_bytes(head_dim)]``, zeros at first).  A group of 32 that holds something not finite
+    reads back as NaN.  Without pools the projection holds queries only."""
+    _need(qkv, torch.float32, "qkv")
+    _need(inv_freq, torch.float32, "inv_freq")
+    _need(q_out, torch.bfloat16, "q_out")
+    if not cache_4bit_supports(q_out.dtype, heads, kv_heads, head_dim):
+        raise KernelError(f"a cache in 4 bits takes head sizes {CACHE_4BIT_DIMS} and up to 16 query heads per key/value head, not {heads}/{kv_heads} heads of {head_dim}")
+    if (k_pool is None) != (v_pool is None):
+        raise KernelError("the pools come as both of keys and values, or neither")
+    write = k_pool is not None
+    cols = (heads + (2 * kv_heads if write else 0)) * head_dim
+    if qkv.dim() != 3 or tuple(qkv.shape[1:]) != (n_tokens, cols):
+        raise KernelError(f"qkv is {tuple(qkv.shape)}, expected [splits, {n_tokens}, {cols}]")
+    if q_out.numel() != n_tokens * heads * head_dim:
+        raise KernelError("q_out does not fit the tokens and heads")
+    if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.numel() < rotary_dim // 2:
+        raise KernelError(f"the rotary part must be even, at most {head_dim} numbers, and have half as many frequencies; got {rotary_dim} and {inv_freq.numel()}")
+    _need_aligned(q_out, "q_out")
+    if write:
+        _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    else:
+        _check_step(table, cu, len_before, sequences, status)
+    fn = _fn("cache_4bit", "tt_rope_append_4bit", "pilpiifppppiippiiiiiipp")
+    _check(fn(_ptr(qkv), qkv.shape[0], qkv.stride(0), _ptr(inv_freq), rotary_dim, 1 if interleaved else 0, attention_scaling, _ptr(q_out), _ptr(k_pool),
+              _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0] if write else 0, _ptr(cu), _ptr(len_before), sequences, n_tokens, heads,
+              kv_heads, head_dim, 1 if write else 0, _ptr(status), _stream()), "rope_append_4bit")
+
+
+def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
+                window: int, keys: torch.Tensor, values: torch.Tensor, table_tmp: torch.Tensor, status: torch.Tensor) -> None:
+    """The blocks of a cache in 4 bits that a step's queries see, as bfloat16 blocks: ``keys`` ``[places, kv_heads, 64, head_dim]`` and ``values``
+    ``[places, kv_heads, head_dim, 64]`` with ``places`` a multiple of ``sequences``: a sequence's blocks, from the first that it sees (``window`` as in
+    :func:`attention`), lie side by side in its ``places / sequences`` places (a step that sees more flags a bad shape), tokens behind its end
+    are zero, and places that it does not fill stay as they are.  ``table_tmp`` (int32, like ``table``) names the place of every block, -1 for those not
+    seen: with it, ``keys`` and ``values`` are what a plain cache's pools and table would be."""
+    _need(keys, torch.bfloat16, "expanded keys")
+    _need(values, torch.bfloat16, "expanded values")
+    _need(table_tmp, torch.int32, "temporary table")
+    if keys.dim() != 4 or keys.shape[2] != BLOCK_TOKENS or keys.shape[3] not in CACHE_4BIT_DIMS:
+        raise KernelError(f"expanded keys must be [places, kv_heads, {BLOCK_TOKENS}, head size], got {tuple(keys.shape)}")
+    places, kv_heads, _, head_dim = keys.shape
+    if tuple(values.shape) != (places, kv_heads, head_dim, BLOCK_TOKENS) or tuple(table_tmp.shape) != tuple(table.shape) or places < sequences or places % sequences:
+        raise KernelError("expand_4bit: values, temporary table or number of places do not fit")
+    _need_aligned(keys, "expanded keys")
+    _need_aligned(values, "expanded values")
+    _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    fn = _fn("cache_4bit", "tt_expand_4bit", "pppiippiiiiippppp")
+    _check(fn(_ptr(k_pool), _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0], _ptr(cu), _ptr(len_before), sequences, kv_heads, head_dim,
+              window, places // sequences, _ptr(keys), _ptr(values), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
+
+
+def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor,
+                   len_before: torch.Tensor, sequences: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int, scale: float,
+                   window: int, splits: int, out: torch.Tensor, part_acc: torch.Tensor | None, part_ml: torch.Tensor | None,
+                   status: torch.Tensor, one_token_each: bool = False, sinks: torch.Tensor | None = None) -> None:
+    """Causal grouped-query attention of packed bfloat16 queries ``q`` [tokens, heads * head_dim] over a cache in 4 bits (see
+    :func:`rope_append_4bit`), into ``out`` of the same shape; ``window`` and ``sinks`` as in :func:`attention`, ``scale`` positive.  ``one_token_each``
+    (decoding): every sequence brings one token.  Any number of tokens is taken, but every few of them read the sequence's cache
+    anew: prompts are faster through :func:`expand_4bit`.  ``splits`` slices the keys; more than 8 need ``part_acc`` (float32
+    [tokens * heads * splits * head_dim]) and ``part_ml`` ([tokens * heads * splits * 2])."""
+    if not cache_4bit_supports(q.dtype, heads, kv_heads, head_dim):
+        raise KernelError(f"attention over 4 bits takes bfloat16, head sizes {CACHE_4BIT_DIMS} and up to 16 query heads per key/value head, not {q.dtype}, "
+                          f"{heads}/{kv_heads} heads of {head_dim}")
+    _need(q, torch.bfloat16, "queries")
+    _need(out, torch.bfloat16, "the output")
+    if q.numel() != n_tokens * heads * head_dim or out.numel() != q.numel():
+        raise KernelError("queries or output do not fit the tokens and heads")
+    if not scale > 0.0:
+        raise KernelError(f"the scale of the scores must be positive, got {scale}")
+    if one_token_each and n_tokens != sequences:
+        raise KernelError("one_token_each needs exactly one token per sequence")
+    if splits < 1 or splits > 65535:
+        raise KernelError(f"keys are cut into 1 to 65535 slices, not {splits}")
+    _need_aligned(q, "queries")
+    _check_sinks(sinks, heads)
+    _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    if splits > 8:
+        for t, count, name in ((part_acc, n_tokens * heads * splits * head_dim, "slice sums"), (part_ml, n_tokens * heads * splits * 2, "slice maxima")):
+            if t is None or t.dtype != torch.float32 or t.numel() < count:
+                raise KernelError(f"attention_4bit: {splits} slices need {count} float32 {name}")
+    wide = not one_token_each and n_tokens > sequences                 # several tokens of a sequence share a pass over its keys
+    fn = _fn("cache_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppppp")
+    _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0], _ptr(cu), _ptr(len_before), sequences, n_tokens,
+              heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, 1 if wide else 0, _ptr(out), _ptr(part_acc), _ptr(part_ml),
+              _ptr(status), _ptr(sinks), _stream()), "attention_4bit", 2 if splits > 8 else 1)
+
+
 # --------------------------------------------------------------------- latent attention
 LATENT_MAX_RANK, LATENT_MAX_ROW, LATENT_MAX_DIM = 512, 1024, 256
 

@@ -41,6 +41,7 @@ SOURCES: dict[str, list[str]] = {
     "attention_forms": [],
     "attention_mma": [],
     "attention_tcgen05": [],
+    "cache_4bit": [],
     "recurrent": [],
     "recurrent_chunks": [],
     "latent_attention": [],

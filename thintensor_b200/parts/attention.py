@@ -166,6 +166,16 @@ class CausalAttention(Mixer):
             return triangle(self.window) + (tokens - self.window) * self.window
         return triangle(tokens)
 
+    def no_4bit_cache(self, dtype) -> str | None:
+        if not api.cache_4bit_supports(dtype, self.heads, self.kv_heads, self.head_dim):
+            return (f"{dtype} with {self.heads}/{self.kv_heads} heads of {self.head_dim} (it takes bfloat16, head sizes "
+                    f"{', '.join(map(str, api.CACHE_4BIT_DIMS))} and up to 16 query heads per key/value head)")
+        options = {"value heads of another size": self.value_dim != self.head_dim, "normed queries and keys": self.qk_norm_eps is not None,
+                   "a convolution": bool(self.conv), "capped scores": self.softcap > 0.0, "a distance bias": self.slope_exponent is not None,
+                   "an output gate": self.gate is not None}
+        has = [name for name, on in options.items() if on]
+        return f"{', '.join(has)}: only its plain form, with sinks or windows, reads 4 bits" if has else None
+
     def state_needs(self) -> list[StateNeed]:
         return [StateNeed((self.conv - 1, self.conv_channels), torch.float32)] if self.conv > 1 else []
 
@@ -228,6 +238,14 @@ class CausalAttention(Mixer):
         q_cols = self.heads * self.head_dim
         rot = self.rot
         mixed = ctx.scratch("attention.mixed", (ctx.n_tokens, self.heads * self.value_dim))
+        if cache.k_pool.dtype == torch.uint8:      # a cache in 4 bits
+            projection = (self.qkv if cache.writes else self.q_only)(ctx, x, "attention.qkv")
+            q = ctx.scratch("attention.q", (ctx.n_tokens, q_cols))
+            api.rope_append_4bit(projection, rot.inv_freq, rot.rotary_dim, rot.attention_scaling, q, cache.k_pool if cache.writes else None,
+                                 cache.v_pool if cache.writes else None, table, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads,
+                                 self.kv_heads, self.head_dim, ctx.status, interleaved=rot.interleaved)
+            self.attend(ctx, q, cache, table, mixed)
+            return self.out.delta(ctx, mixed, "attention.out")
         if self.general:
             if cache.writes != self.own_keys and (self.gate or self.conv or not self.own_keys):
                 raise RuntimeError("an attention layer writes the cache exactly when it projects keys and values of its own")
@@ -318,6 +336,51 @@ class CausalAttention(Mixer):
             return None
         return ctx.workspace.get_zeroed("attention.tickets", (max(ctx.sequences * self.kv_heads, 64),), torch.int32)
 
+    # ------------------------------------------------------------------ a cache in 4 bits
+    EXPAND_4BIT_FROM = 16           # new tokens a sequence (on average) from which a step's blocks are expanded
+    EXPAND_4BIT_BYTES = 4 << 30     # most scratch memory that the expanded blocks may take
+
+    def span_4bit(self, ctx, width: int) -> int:
+        """Blocks that a sequence of the step can see, from the step's shape alone (a replayed step has other lengths): all of
+        its table, or what its new tokens and the window or chunk before them can touch."""
+        bound = self.window or self.chunk
+        if not bound:
+            return width
+        return min(width, (ctx.n_tokens - ctx.sequences + 1 + bound - 1 + 62) // 64 + 1)
+
+    def expands_4bit(self, ctx, width: int) -> bool:
+        """Whether a step's prompts go through bfloat16 copies of the blocks that they see: the 4-bit kernel reads a sequence's cache
+        once for every few tokens, the copies are read by kernels that take a hundred at a time (with sinks: the tcgen05 kernel alone)."""
+        if ctx.decode or ctx.n_tokens < self.EXPAND_4BIT_FROM * ctx.sequences:
+            return False
+        if self.sinks is not None and not api.attention_tcgen05_supports(torch.bfloat16, self.heads, self.kv_heads, self.head_dim):
+            return False
+        return ctx.sequences * self.span_4bit(ctx, width) * 64 * self.kv_heads * self.head_dim * 4 <= self.EXPAND_4BIT_BYTES
+
+    def attend_4bit(self, ctx, q, cache, table, mixed) -> None:
+        width = table.shape[1]
+        if self.expands_4bit(ctx, width):
+            places = ctx.sequences * self.span_4bit(ctx, width)
+            keys = ctx.scratch("attention.keys", (places, self.kv_heads, 64, self.head_dim))
+            values = ctx.scratch("attention.values", (places, self.kv_heads, self.head_dim, 64))
+            named = ctx.scratch("attention.table", tuple(table.shape), torch.int32)
+            api.expand_4bit(cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, self.reach, keys, values, named, ctx.status)
+            if api.attention_tcgen05_supports(q.dtype, self.heads, self.kv_heads, self.head_dim):
+                api.attention_tcgen05(q, keys, values, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
+                                      self.head_dim, self.scale, self.reach, mixed, ctx.status, sinks=self.sinks)
+            else:
+                api.attention_mma(q, keys, values, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
+                                  self.head_dim, self.scale, self.reach, 1, mixed, None, None, ctx.status)
+            return
+        # slices of the keys until the CTAs fill the GPU, each of 512 keys at least
+        tiles = ctx.sequences if ctx.decode else -(-ctx.n_tokens * (self.heads // self.kv_heads) // 16)
+        bound = min(ctx.max_total, self.window or self.chunk or ctx.max_total)
+        splits = max(1, min(api.sm_count(ctx.status.device) // max(1, tiles * self.kv_heads), bound // 512, 64))
+        part_acc, part_ml = self.slice_scratch(ctx, splits) if splits > 8 else (None, None)
+        api.attention_4bit(q, cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
+                           self.head_dim, self.scale, self.reach, splits, mixed, part_acc, part_ml, ctx.status, one_token_each=ctx.decode,
+                           sinks=self.sinks)
+
     TENSOR_CORES_FROM = 1           # packed tokens from which prompts run the tcgen05 kernel
 
     @property
@@ -329,7 +392,11 @@ class CausalAttention(Mixer):
         """Prompts in bfloat16 with head size 64 or 128: the tcgen05 kernel.  Other bfloat16
         sizes up to 128 and all decoding: the mma.sync kernels.  Everything else (float32,
         head sizes 48, 80, 144 ..., values of another size than the keys): the exact kernel.
-        Sinks go with the tcgen05 prompt kernel, the mma.sync decode kernel and the exact kernel."""
+        Sinks go with the tcgen05 prompt kernel, the mma.sync decode kernel and the exact kernel.
+        A cache in 4 bits has its own kernel and, for prompts, its blocks expanded for the prompt kernels."""
+        if cache.k_pool.dtype == torch.uint8:
+            self.attend_4bit(ctx, q, cache, table, mixed)
+            return
         same = self.value_dim == self.head_dim
         if (same and not ctx.decode and ctx.n_tokens >= self.TENSOR_CORES_FROM
                 and api.attention_tcgen05_supports(q.dtype, self.heads, self.kv_heads, self.head_dim)):

@@ -72,10 +72,16 @@ class KVNeed:
     window: int | None = None
     value_dim: int | None = None        # numbers per value head where they differ from the keys' (None: head_dim)
     every: int = 1                      # one entry for each ``every`` tokens: entry n belongs to tokens n * every .. n * every + every - 1
+    bits: int | None = None             # 4: codes of 4 bits with a scale and a least value for each 32 numbers of a head; None: the engine's type
 
     @property
     def v_dim(self) -> int:
         return self.head_dim if self.value_dim is None else self.value_dim
+
+    def token_bytes(self, dtype: torch.dtype) -> int:
+        """Bytes that a token's keys and values (or an entry's, with ``every``) take in a cache of an engine of this type."""
+        numbers = self.kv_heads * (self.head_dim + self.v_dim)
+        return numbers * 5 // 8 if self.bits == 4 else numbers * torch.empty((), dtype=dtype).element_size()
 
 
 @dataclass(frozen=True)
@@ -240,6 +246,10 @@ class Mixer(Part):
         """A second, coarser cache beside the mixer's keys and values: one key and one value for each ``every`` tokens
         (the means of whole blocks of tokens, say).  ``forward`` finds it as ``cache.summary``."""
         return None
+
+    def no_4bit_cache(self, dtype: torch.dtype) -> str | None:
+        """Why the mixer cannot keep its keys and values in 4 bits (None: it can; ``forward`` then meets pools of bytes)."""
+        return "its kernels read a cache in the engine's type"
 
     def state_needs(self) -> list[StateNeed]:
         """Per-sequence state tensors of fixed size, zero when a sequence starts; ``forward`` gets
