@@ -314,23 +314,34 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
 // ------------------------------------------------------------------------------------------------------------- attention
 // With codes n, scales s and least values m of key t and value t (primes for values), per group g:
 //   score(q, t) = sum_g s_tg (q . n)_tg + m_tg (sum of q over g),     out_g = sum_t (p_t s'_tg) n'_t + p_t m'_tg.
-// So the tensor cores multiply codes, not numbers: an operand register is a shift and a mask away from the cache's words, scales meet
-// the 16 x 8 tile of a group's products (S^T: 16 keys, 8 queries) and the probabilities.
+// So the tensor cores multiply codes, not numbers.  As float16 the bits 0x000n are n 2^-24 and 0x00n0 are 16 n 2^-24 (numbers below the
+// normal ones, which the tensor cores take as they are): an operand register of two codes is one mask away from the cache's word, and
+// eight codes take one shift and four masks.  What the sixteens multiply is a sixteenth (queries) or is taken off the sums' rows
+// (values), the 2^24 goes into the scale.  Group scales meet the 16 x 8 tile of a group's products (S^T: 16 keys, 8 queries) and the
+// probabilities; the least values are one more product of each, in bfloat16.
 //
-// S: bfloat16 operands 128 + n and the queries as they are; what the 128s add is known (128 sum q), and the accumulator starts at minus
-// that.  Exact but for float32 sums.
-// O: the weights p s' are rounded to float16 (11 bits), the codes are float16 whole numbers: with weights in bfloat16 the two terms,
-// which are of opposite sign and each several times the sum, were off by 0.4 % of it; and 128s left in the operands would cost as much
-// again where thousands of keys average out.  So that float16 holds them whatever the values' size, p is formed relative to the running
-// maximum times 2^(E - 14), E the exponent of the largest scale that the warp has met (at least -40): the weights stay below 2^15, and
-// what falls under 2^-14 is less than 2^-29 of the largest.  The second term takes p in two bfloat16 parts (16 bits) and m' as it is.
-// All sums are float32.
+// Queries are float16 after a power of two that brings a row's greatest number to 2^14: exact but for what lies 2^-28 below that.
+// The weights p s' are rounded to float16 (11 bits): with weights in bfloat16 the two terms of out, which are of opposite sign and
+// each several times their sum, were off by 0.4 % of it.  So that float16 holds them whatever the values' size, p is formed relative to
+// the running maximum times 2^(E - 14), E the exponent of the largest scale that the warp has met (at least -40): the weights stay
+// below 2^15, and what falls under 2^-14 is less than 2^-29 of the largest.  The second term takes p in two bfloat16 parts (16 bits)
+// and m' as it is, the second term of S the queries' sums in three.  All sums are float32.
+//
+// Rows of up to four queries (DUP) stand twice in the tile's eight columns, which would otherwise be half empty: the weights of one
+// group of numbers lie in the first four, those of the next group in the others, and the products of either group take the same
+// operand.
 //
 // A warp owns up to 8 NQ query rows of one sequence and key/value head, (token, head of the group) pairs, and walks its share of the
 // blocks; the copy engine brings a block's keys and values (5 KB each at D = 128) into its ring of shared-memory stages a block ahead.
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -343,7 +354,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// 2^x on the special-function unit (relative error about 2^-22), 2^-inf = 0; what it gives is rounded to bfloat16 or summed beside that.
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// 2^x on the special-function unit (relative error about 2^-22), 2^-inf = 0; what it gives is rounded to float16 or summed beside that.
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -353,26 +370,8 @@ __device__ __forceinline__ void bulk_copy(void* smem_dst, const void* src, uint3
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(tc::smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Two codes of a word as bfloat16 numbers 128 + n.
-template <int I> __device__ __forceinline__ uint32_t codes(uint32_t w) { return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u; }
-// The same as float16 whole numbers: n of the codes at bits 0 and 16, 16 n of those at bits 4 and 20 (1024 and 1024 taken off).
-__device__ __forceinline__ uint32_t less_1024(uint32_t v) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0x64006400u));
-    return d;
-}
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) { return less_1024((w & 0x000f000fu) | 0x64006400u); }
-__device__ __forceinline__ uint32_t codes_f16_by_16(uint32_t w) { return less_1024((w & 0x00f000f0u) | 0x64006400u); }
+constexpr uint32_t ONES_MASK = 0x000f000fu, SIXTEENS_MASK = 0x00f000f0u;       // codes n and 16 n of a word
+constexpr float CODE_UNIT = 5.9604644775390625e-08f;                            // 2^-24
 
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     if constexpr (N == 4) {
@@ -387,78 +386,90 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
     }
 }
 
-template <int D, int NQ> struct Rows4 {
+template <int D, int NQ, bool DUP> struct Rows4 {
     static constexpr int G = D / 32;
-    uint32_t q[NQ][G][4];               // query 8 nq + r: numbers 32 g + 8 c + 2 i and + 1 in register i
-    float q_sum[NQ][G][2];              // sums of queries 8 nq + 2 c + e over a group
+    uint32_t q[NQ][G][4];               // query 8 nq + r: numbers 32 g + 8 c + 2 i and + 1 in register i, float16, those of odd i a sixteenth
+    uint32_t q_sum[NQ][2];              // the sum of query 8 nq + r over group c, in three bfloat16 parts
     float o[2 * G][NQ][4];              // [0], [1]: number 16 dt + r, queries 8 nq + 2 c + e; [2], [3]: number + 8, sixteenfold
     float least[NQ][4];                 // row r = group r: the least values' share
+    float scale[NQ][2];                 // of the scores of queries 8 nq + 2 c + e, in log2 units
     float m_run[NQ][2], l_run[NQ][2];   // l: this lane's share (its keys) until the end
     int e_run;                          // E: all weights and sums are relative to 2^(m_run + E - 14)
     int pos[NQ][2], first[NQ][2];       // queries 8 nq + 2 c + e see keys first .. pos
 };
 
-template <int D, int NQ>
-__device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* __restrict__ kb, const uint8_t* __restrict__ vb, int key_base,
-                                              bool all_visible, int first_seen, int last_pos, int r, int c, float scale_log2) {
-    constexpr int G = Rows4<D, NQ>::G;
+template <int D, int NQ, bool DUP>
+__device__ __forceinline__ void block_of_keys(Rows4<D, NQ, DUP>& st, const uint8_t* __restrict__ kb, const uint8_t* __restrict__ vb, int key_base,
+                                              bool all_visible, int first_seen, int last_pos, int r, int c) {
+    constexpr int G = Rows4<D, NQ, DUP>::G;
     const int lane = 4 * r + c;
     const int token0 = 4 * (r >> 1) + (r & 1);                         // rows r and r + 8 of a tile of 16 keys: tokens token0 and + 2
     float s[4][NQ][4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
         const int t0 = 16 * kt + token0;
+        const uint8_t* pairs = kb + code_bytes(D) + t0 * 4 * G;
         uint32_t w0[G], w1[G], p0[G], p1[G];
         load_words<G>(kb + (t0 * 4 + c) * 4 * G, w0);
         load_words<G>(kb + ((t0 + 2) * 4 + c) * 4 * G, w1);
-        load_words<G>(kb + code_bytes(D) + t0 * 4 * G, p0);
-        load_words<G>(kb + code_bytes(D) + (t0 + 2) * 4 * G, p1);
+        load_words<G>(pairs, p0);
+        load_words<G>(pairs + 8 * G, p1);
+        // the least values of group c, twice in a register
+        const uint32_t m0 = c < G ? __byte_perm(reinterpret_cast<const uint32_t*>(pairs)[c < G ? c : 0], 0u, 0x3232) : 0u;
+        const uint32_t m1 = c < G ? __byte_perm(reinterpret_cast<const uint32_t*>(pairs + 8 * G)[c < G ? c : 0], 0u, 0x3232) : 0u;
 #pragma unroll
-        for (int nq = 0; nq < NQ; ++nq) s[kt][nq][0] = s[kt][nq][1] = s[kt][nq][2] = s[kt][nq][3] = 0.0f;
+        for (int nq = 0; nq < NQ; ++nq) {
+            s[kt][nq][0] = s[kt][nq][1] = s[kt][nq][2] = s[kt][nq][3] = 0.0f;
+            mma_bf16(s[kt][nq], m0, m1, m0, m1, st.q_sum[nq][0], st.q_sum[nq][1]);
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const uint32_t a0 = codes<0>(w0[g]), a1 = codes<0>(w1[g]), a2 = codes<1>(w0[g]), a3 = codes<1>(w1[g]);
-            const uint32_t a4 = codes<2>(w0[g]), a5 = codes<2>(w1[g]), a6 = codes<3>(w0[g]), a7 = codes<3>(w1[g]);
-            const float s0 = __uint_as_float(p0[g] << 16), m0 = __uint_as_float(p0[g] & 0xffff0000u);
-            const float s1 = __uint_as_float(p1[g] << 16), m1 = __uint_as_float(p1[g] & 0xffff0000u);
+            const uint32_t h0 = w0[g] >> 8, h1 = w1[g] >> 8;
+            const float s0 = bf16_low(p0[g]), s1 = bf16_low(p1[g]);
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
-                const float x0 = st.q_sum[nq][g][0], x1 = st.q_sum[nq][g][1];
-                float acc[4] = {-128.0f * x0, -128.0f * x1, -128.0f * x0, -128.0f * x1};
-                mma_bf16(acc, a0, a1, a2, a3, st.q[nq][g][0], st.q[nq][g][1]);
-                mma_bf16(acc, a4, a5, a6, a7, st.q[nq][g][2], st.q[nq][g][3]);
-                s[kt][nq][0] = fmaf(s0, acc[0], fmaf(m0, x0, s[kt][nq][0]));
-                s[kt][nq][1] = fmaf(s0, acc[1], fmaf(m0, x1, s[kt][nq][1]));
-                s[kt][nq][2] = fmaf(s1, acc[2], fmaf(m1, x0, s[kt][nq][2]));
-                s[kt][nq][3] = fmaf(s1, acc[3], fmaf(m1, x1, s[kt][nq][3]));
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_f16(acc, w0[g] & ONES_MASK, w1[g] & ONES_MASK, w0[g] & SIXTEENS_MASK, w1[g] & SIXTEENS_MASK, st.q[nq][g][0], st.q[nq][g][1]);
+                mma_f16(acc, h0 & ONES_MASK, h1 & ONES_MASK, h0 & SIXTEENS_MASK, h1 & SIXTEENS_MASK, st.q[nq][g][2], st.q[nq][g][3]);
+                s[kt][nq][0] = fmaf(s0, acc[0], s[kt][nq][0]);
+                s[kt][nq][1] = fmaf(s0, acc[1], s[kt][nq][1]);
+                s[kt][nq][2] = fmaf(s1, acc[2], s[kt][nq][2]);
+                s[kt][nq][3] = fmaf(s1, acc[3], s[kt][nq][3]);
             }
         }
     }
-    if (!all_visible) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) {
-                const int key = key_base + 16 * kt + token0 + 2 * hi;
-#pragma unroll
-                for (int nq = 0; nq < NQ; ++nq)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (!(key <= st.pos[nq][e] && key >= st.first[nq][e])) s[kt][nq][2 * hi + e] = -INFINITY;
-            }
-    }
     const uint8_t* scales = vb + code_bytes(D);
     const uint8_t* mins = scales + 2 * TT_BLOCK_TOKENS * G;
-    // the exponent of the block's largest scale: a lane looks at two neighbouring tokens (bits of positive bfloat16 numbers order like them)
+    // the bits of the block's largest scale: a lane looks at two neighbouring tokens (positive bfloat16 numbers order like their bits; a scale
+    // that is not a number counts for nothing here)
     uint32_t top = 0u;
     {
         uint32_t two[G];
         load_words<G>(scales + 2 * lane * 2 * G, two);
+        if (all_visible) {
+            __nv_bfloat162 most = *reinterpret_cast<const __nv_bfloat162*>(&two[0]);
 #pragma unroll
-        for (int i = 0; i < 2 * G; ++i) {
-            const uint32_t bits = (two[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            const int key = key_base + 2 * lane + i / G;
-            if (bits <= 0x7f80u && (all_visible || (key <= last_pos && key >= first_seen))) top = max(top, bits);
+            for (int i = 1; i < G; ++i) most = __hmax2(most, *reinterpret_cast<const __nv_bfloat162*>(&two[i]));
+            const uint32_t bits = *reinterpret_cast<const uint32_t*>(&most), lo = bits & 0xffffu, hi = bits >> 16;
+            top = max(lo <= 0x7f80u ? lo : 0u, hi <= 0x7f80u ? hi : 0u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i) {
+                const uint32_t bits = (two[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+                const int key = key_base + 2 * lane + i / G;
+                if (bits <= 0x7f80u && key <= last_pos && key >= first_seen) top = max(top, bits);
+            }
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int hi = 0; hi < 2; ++hi) {
+                    const int key = key_base + 16 * kt + token0 + 2 * hi;
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (!(key <= st.pos[nq][e] && key >= st.first[nq][e])) s[kt][nq][2 * hi + e] = -INFINITY;
+                }
         }
     }
     const int e_new = max(st.e_run, (int)(__reduce_max_sync(0xffffffffu, top) >> 7) - 127);
@@ -476,7 +487,7 @@ __device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* _
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(st.m_run[nq][e], mx * scale_log2);         // the scale is positive
+            const float m_new = fmaxf(st.m_run[nq][e], mx * st.scale[nq][e]);         // the scale is positive
             corr[nq][e] = m_new == -INFINITY ? 1.0f : fast_exp2((st.m_run[nq][e] - m_new) + (e_old - e_now));
             grew = grew || corr[nq][e] != 1.0f;
             const float base = m_new == -INFINITY ? 0.0f : -(m_new + e_now);
@@ -485,7 +496,7 @@ __device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* _
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                 for (int hi = 0; hi < 2; ++hi) {
-                    const float p = fast_exp2(fmaf(s[kt][nq][2 * hi + e], scale_log2, base));
+                    const float p = fast_exp2(fmaf(s[kt][nq][2 * hi + e], st.scale[nq][e], base));
                     s[kt][nq][2 * hi + e] = p;
                     sum += p;
                 }
@@ -504,6 +515,7 @@ __device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* _
             st.least[nq][0] *= corr[nq][0]; st.least[nq][1] *= corr[nq][1];
         }
     }
+    constexpr int SETS = DUP ? (G + 1) / 2 : G;                        // operands of weights: with DUP one holds two groups'
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
         const int t0 = 16 * kt + token0;
@@ -519,20 +531,26 @@ __device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* _
         }
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
-            const uint32_t hi0 = pack_bf16(s[kt][nq][0], s[kt][nq][1]), hi1 = pack_bf16(s[kt][nq][2], s[kt][nq][3]);
-            const uint32_t lo0 = pack_bf16(s[kt][nq][0] - __uint_as_float(hi0 << 16), s[kt][nq][1] - __uint_as_float(hi0 & 0xffff0000u));
-            const uint32_t lo1 = pack_bf16(s[kt][nq][2] - __uint_as_float(hi1 << 16), s[kt][nq][3] - __uint_as_float(hi1 & 0xffff0000u));
-            mma_bf16(st.least[nq], low.x, 0u, low.y, 0u, transpose_8x8(hi0), transpose_8x8(hi1));
-            mma_bf16(st.least[nq], low.x, 0u, low.y, 0u, transpose_8x8(lo0), transpose_8x8(lo1));
-        }
+            float rest[4];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float s0 = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(scales)[t0 * G + g]);
-            const float s1 = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(scales)[(t0 + 2) * G + g]);
-            const uint2 w = *reinterpret_cast<const uint2*>(vb + ((kt * G + g) * 32 + lane) * 8);
-            const uint32_t x8 = w.x >> 8, y8 = w.y >> 8;
-            const uint32_t x0 = codes_f16(w.x), x1 = codes_f16_by_16(w.x), x2 = codes_f16(x8), x3 = codes_f16_by_16(x8);
-            const uint32_t y0 = codes_f16(w.y), y1 = codes_f16_by_16(w.y), y2 = codes_f16(y8), y3 = codes_f16_by_16(y8);
+            for (int i = 0; i < 4; ++i) rest[i] = s[kt][nq][i] - bf16_high(__float_as_uint(s[kt][nq][i]));
+            if constexpr (DUP) {                                       // the first part in the first four columns, the second in the others
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rest[i] = c < 2 ? bf16_high(__float_as_uint(s[kt][nq][i])) : rest[i];
+                mma_bf16(st.least[nq], low.x, 0u, low.y, 0u, transpose_8x8(pack_bf16(rest[0], rest[1])), transpose_8x8(pack_bf16(rest[2], rest[3])));
+            } else {
+                const uint32_t hi0 = __byte_perm(__float_as_uint(s[kt][nq][0]), __float_as_uint(s[kt][nq][1]), 0x7632);
+                const uint32_t hi1 = __byte_perm(__float_as_uint(s[kt][nq][2]), __float_as_uint(s[kt][nq][3]), 0x7632);
+                mma_bf16(st.least[nq], low.x, 0u, low.y, 0u, transpose_8x8(hi0), transpose_8x8(hi1));
+                mma_bf16(st.least[nq], low.x, 0u, low.y, 0u, transpose_8x8(pack_bf16(rest[0], rest[1])), transpose_8x8(pack_bf16(rest[2], rest[3])));
+            }
+        }
+        const __nv_bfloat16* scale0 = reinterpret_cast<const __nv_bfloat16*>(scales) + t0 * G;
+#pragma unroll
+        for (int set = 0; set < SETS; ++set) {
+            const int mine = DUP ? min(2 * set + (c >> 1), G - 1) : set;       // the group whose weights this lane forms
+            const float s0 = __bfloat162float(scale0[mine]), s1 = __bfloat162float(scale0[2 * G + mine]);
+            uint32_t b0[NQ], b1[NQ];
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
                 float p0 = s[kt][nq][0] * s0, p1 = s[kt][nq][1] * s0, p2 = s[kt][nq][2] * s1, p3 = s[kt][nq][3] * s1;
@@ -540,9 +558,18 @@ __device__ __forceinline__ void block_of_keys(Rows4<D, NQ>& st, const uint8_t* _
                     p0 = s[kt][nq][0] == 0.0f ? 0.0f : p0; p1 = s[kt][nq][1] == 0.0f ? 0.0f : p1;
                     p2 = s[kt][nq][2] == 0.0f ? 0.0f : p2; p3 = s[kt][nq][3] == 0.0f ? 0.0f : p3;
                 }
-                const uint32_t b0 = transpose_8x8(pack_f16(p0, p1)), b1 = transpose_8x8(pack_f16(p2, p3));
-                mma_f16(st.o[2 * g][nq], x0, x1, x2, x3, b0, b1);
-                mma_f16(st.o[2 * g + 1][nq], y0, y1, y2, y3, b0, b1);
+                b0[nq] = transpose_8x8(pack_f16(p0, p1));
+                b1[nq] = transpose_8x8(pack_f16(p2, p3));
+            }
+#pragma unroll
+            for (int g = DUP ? 2 * set : set; g < (DUP ? min(2 * set + 2, G) : set + 1); ++g) {
+                const uint2 w = *reinterpret_cast<const uint2*>(vb + ((kt * G + g) * 32 + lane) * 8);
+                const uint32_t x8 = w.x >> 8, y8 = w.y >> 8;
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) {
+                    mma_f16(st.o[2 * g][nq], w.x & ONES_MASK, w.x & SIXTEENS_MASK, x8 & ONES_MASK, x8 & SIXTEENS_MASK, b0[nq], b1[nq]);
+                    mma_f16(st.o[2 * g + 1][nq], w.y & ONES_MASK, w.y & SIXTEENS_MASK, y8 & ONES_MASK, y8 & SIXTEENS_MASK, b0[nq], b1[nq]);
+                }
             }
         }
     }
@@ -558,7 +585,7 @@ template <int D> struct Ring4 {
 };
 
 // grid = (tiles, kv_heads, splits).  tokens_per_tile 1 with one token a sequence: tile = sequence.
-template <int D, int NQ>
+template <int D, int NQ, bool DUP>
 __global__ void __launch_bounds__(Ring4<D>::WARPS * 32)
 attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool,
                       const int* __restrict__ table, int table_width, int pool_blocks, const int* __restrict__ cu,
@@ -644,32 +671,56 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
     };
     while (issued < min(n_mine, STAGES)) issue_next();
 
-    Rows4<D, NQ> st;
+    Rows4<D, NQ, DUP> st;
     st.e_run = -40;
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
-        const int row = 8 * nq + r;
-        const __nv_bfloat16* src = q + ((size_t)(seq_begin + tok0 + row / group) * heads + kh * group + row % group) * D;
+        const int row = DUP ? r & 3 : 8 * nq + r;
+        const __nv_bfloat16* src = q + ((size_t)(seq_begin + tok0 + row / group) * heads + kh * group + row % group) * D + 8 * c;
+        uint4 v[G];
+        uint32_t most = 0u;                                            // bits of the row's greatest number without its sign
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const uint4 v = row < n_rows ? *reinterpret_cast<const uint4*>(src + 32 * g + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-            st.q[nq][g][0] = v.x; st.q[nq][g][1] = v.y; st.q[nq][g][2] = v.z; st.q[nq][g][3] = v.w;
+            v[g] = row < n_rows ? *reinterpret_cast<const uint4*>(src + 32 * g) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = max(most, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+        }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // times 2^up: the greatest number's exponent becomes 14
+        const int up = max(min(141 - (int)(most >> 23), 120), -100);
+        const float factor = __uint_as_float((uint32_t)(127 + up) << 23);
+        uint32_t parts[2] = {0u, 0u};
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sum += __uint_as_float(st.q[nq][g][i] << 16) + __uint_as_float(st.q[nq][g][i] & 0xffff0000u);
+            for (int i = 0; i < 4; ++i) {
+                const float a = bf16_low(w[i]) * factor, b = bf16_high(w[i]) * factor, less = i & 1 ? 0.0625f : 1.0f;
+                sum += a + b;
+                st.q[nq][g][i] = pack_f16(a * less, b * less);
+            }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) st.q_sum[nq][g][e] = __shfl_sync(0xffffffffu, sum, 4 * (2 * c + e));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[2 * g][nq][e] = st.o[2 * g + 1][nq][e] = 0.0f;
+            if (c == g) {                                              // in units of the codes', in three parts
+                sum *= CODE_UNIT;
+                const float hi = __bfloat162float(__float2bfloat16_rn(sum)), mid = __bfloat162float(__float2bfloat16_rn(sum - hi));
+                parts[0] = pack_bf16(hi, mid);
+                parts[1] = pack_bf16(sum - hi - mid, 0.0f);
+            }
         }
+        st.q_sum[nq][0] = parts[0];
+        st.q_sum[nq][1] = parts[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st.least[nq][e] = 0.0f;
+        for (int dt = 0; dt < 2 * G; ++dt) st.o[dt][nq][0] = st.o[dt][nq][1] = st.o[dt][nq][2] = st.o[dt][nq][3] = 0.0f;
+        st.least[nq][0] = st.least[nq][1] = st.least[nq][2] = st.least[nq][3] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int col = 8 * nq + 2 * c + e, local = col / group;
+            const int col = DUP ? (2 * c + e) & 3 : 8 * nq + 2 * c + e, local = col / group;
+            const int back = __shfl_sync(0xffffffffu, up, 4 * (2 * c + e));
+            st.scale[nq][e] = scale_log2 * __uint_as_float((uint32_t)(127 + 24 - back) << 23);
             st.m_run[nq][e] = -INFINITY;
             st.l_run[nq][e] = 0.0f;
             st.pos[nq][e] = col < n_rows ? pos0 + local : -1;
@@ -691,14 +742,14 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             const uint8_t* src = ring + (size_t)(i % STAGES) * R::STAGE;
             const int key_base = (begin + warp + i * WARPS) * TT_BLOCK_TOKENS;
             const bool all_visible = key_base + TT_BLOCK_TOKENS - 1 <= pos0 && key_base >= last_first;
-            block_of_keys<D, NQ>(st, src, src + block_bytes(D), key_base, all_visible, first_key, last_pos, r, c, scale_log2);
+            block_of_keys<D, NQ, DUP>(st, src, src + block_bytes(D), key_base, all_visible, first_key, last_pos, r, c);
         }
         __syncwarp();                                                  // every lane has read the stage
         if (issued < n_mine) issue_next();
     }
     for (int i = waited; i < issued; ++i) tc::mbar_wait(tc::smem_u32(&landed[warp][i % STAGES]), (uint32_t)((i / STAGES) & 1));
 
-    // the least values in, the lanes' shares of the row sums together
+    // the lanes' shares of the row sums together; the codes' unit out, the least values in
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
@@ -708,11 +759,15 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             st.l_run[nq][e] = l;
+            if constexpr (DUP) st.least[nq][e] += __shfl_xor_sync(0xffffffffu, st.least[nq][e], 2);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const float add = __shfl_sync(0xffffffffu, st.least[nq][e], 4 * g + c);
-                st.o[2 * g][nq][e] += add; st.o[2 * g][nq][2 + e] = fmaf(st.o[2 * g][nq][2 + e], 0.0625f, add);
-                st.o[2 * g + 1][nq][e] += add; st.o[2 * g + 1][nq][2 + e] = fmaf(st.o[2 * g + 1][nq][2 + e], 0.0625f, add);
+#pragma unroll
+                for (int dt = 2 * g; dt < 2 * g + 2; ++dt) {
+                    st.o[dt][nq][e] = fmaf(st.o[dt][nq][e], 1.0f / CODE_UNIT, add);
+                    st.o[dt][nq][2 + e] = fmaf(st.o[dt][nq][2 + e], 0.0625f / CODE_UNIT, add);
+                }
             }
         }
 
@@ -726,11 +781,15 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
     for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int col = 8 * nq + 2 * c + e;
+            const int col = DUP ? (2 * c + e) & 3 : 8 * nq + 2 * c + e;
             float* dst = sh_o + ((size_t)warp * COLS + col) * PITCH + r;
 #pragma unroll
-            for (int dt = 0; dt < 2 * G; ++dt) { dst[16 * dt] = st.o[dt][nq][e]; dst[16 * dt + 8] = st.o[dt][nq][2 + e]; }
-            if (r == 0) { sh_m[warp * COLS + col] = st.m_run[nq][e] + (float)(st.e_run - 14); sh_l[warp * COLS + col] = st.l_run[nq][e]; }
+            for (int dt = 0; dt < 2 * G; ++dt)
+                if (!DUP || ((dt >> 1) & 1) == (c >> 1)) { dst[16 * dt] = st.o[dt][nq][e]; dst[16 * dt + 8] = st.o[dt][nq][2 + e]; }
+            if (r == 0 && (!DUP || c < 2)) {
+                sh_m[warp * COLS + col] = st.m_run[nq][e] + (float)(st.e_run - 14);
+                sh_l[warp * COLS + col] = st.l_run[nq][e];
+            }
         }
     __syncthreads();
     float* cta_acc = sh_l + WARPS * COLS;                              // [COLS][D]
@@ -805,15 +864,15 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
     }
 }
 
-template <int D, int NQ>
+template <int D, int NQ, bool DUP>
 cudaError_t launch_attention(const void* q, const uint8_t* k_pool, const uint8_t* v_pool, const int* table, int table_width, int pool_blocks,
                              const int* cu, const int* len_before, int sequences, int n_tokens, int heads, int kv_heads, float scale, int window,
                              int splits, int one_token_each, void* out, float* part_acc, float* part_ml, unsigned* status, const float* sinks,
                              cudaStream_t stream) {
-    const int group = heads / kv_heads, tokens_per_tile = one_token_each ? 1 : 8 * NQ / group;
+    const int group = heads / kv_heads, tokens_per_tile = one_token_each ? 1 : (DUP ? 4 : 8 * NQ) / group;
     const int tiles = one_token_each ? sequences : n_tokens / tokens_per_tile + sequences;
     constexpr int shared = Ring4<D>::shared(8 * NQ);
-    auto kernel = attention_4bit_kernel<D, NQ>;
+    auto kernel = attention_4bit_kernel<D, NQ, DUP>;
     const cudaError_t err = tt_allow_shared(kernel, shared);
     if (err != cudaSuccess) return err;
     const bool cluster = splits > 1 && splits <= 8;
@@ -903,12 +962,13 @@ extern "C" int tt_attention_4bit(const void* q, const void* k_pool, const void* 
         (splits > 8 && (!part_acc || !part_ml)))
         return (int)cudaErrorInvalidValue;
     const int group = heads / kv_heads;
-#define TT_LAUNCH(D, NQ)                                                                                                                    \
-    return (int)launch_attention<D, NQ>(q, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, cu, len_before, sequences, \
-                                        n_tokens, heads, kv_heads, scale, window, splits, one_token_each, out, part_acc, part_ml, status, sinks, stream)
-#define TT_LAUNCH_D(D)                       \
-    if (group > 8 || wide) TT_LAUNCH(D, 2); \
-    TT_LAUNCH(D, 1)
+#define TT_LAUNCH(D, NQ, DUP)                                                                                                                    \
+    return (int)launch_attention<D, NQ, DUP>(q, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, cu, len_before, sequences, \
+                                             n_tokens, heads, kv_heads, scale, window, splits, one_token_each, out, part_acc, part_ml, status, sinks, stream)
+#define TT_LAUNCH_D(D)                              \
+    if (group > 8 || wide) TT_LAUNCH(D, 2, false); \
+    if (group > 4) TT_LAUNCH(D, 1, false);         \
+    TT_LAUNCH(D, 1, true)
     switch (head_dim) {
         case 32: TT_LAUNCH_D(32);
         case 64: TT_LAUNCH_D(64);
