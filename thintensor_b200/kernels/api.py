@@ -1331,15 +1331,23 @@ def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
               window, places // sequences, _ptr(keys), _ptr(values), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
 
 
+def attention_4bit_part_rows(device: torch.device | int | None = None) -> int:
+    """Rows of scratch memory that :func:`attention_4bit` wants for even runs: two for each query row of a tile and each CTA of the device."""
+    return 64 * sm_count(device)
+
+
 def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor,
                    len_before: torch.Tensor, sequences: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int, scale: float,
                    window: int, splits: int, out: torch.Tensor, part_acc: torch.Tensor | None, part_ml: torch.Tensor | None,
-                   status: torch.Tensor, one_token_each: bool = False, sinks: torch.Tensor | None = None) -> None:
+                   status: torch.Tensor, one_token_each: bool = False, sinks: torch.Tensor | None = None,
+                   tickets: torch.Tensor | None = None) -> None:
     """Causal grouped-query attention of packed bfloat16 queries ``q`` [tokens, heads * head_dim] over a cache in 4 bits (see
     :func:`rope_append_4bit`), into ``out`` of the same shape; ``window`` and ``sinks`` as in :func:`attention`, ``scale`` positive.  ``one_token_each``
     (decoding): every sequence brings one token.  Any number of tokens is taken, but every few of them read the sequence's cache
-    anew: prompts are faster through :func:`expand_4bit`.  ``splits`` slices the keys; more than 8 need ``part_acc`` (float32
-    [tokens * heads * splits * head_dim]) and ``part_ml`` ([tokens * heads * splits * 2])."""
+    anew: prompts are faster through :func:`expand_4bit`.  ``splits`` 1 to 8 cuts the keys of a sequence into so many slices; 0 gives every
+    CTA that the device holds an equal run of all sequences' blocks, whose parts need the float32 scratch ``part_acc``
+    [:func:`attention_4bit_part_rows` * head_dim] and ``part_ml`` [the same * 2], and ``tickets``: int32, four for each multiprocessor, zero before the
+    call and after it."""
     if not cache_4bit_supports(q.dtype, heads, kv_heads, head_dim):
         raise KernelError(f"attention over 4 bits takes bfloat16, head sizes {CACHE_4BIT_DIMS} and up to 16 query heads per key/value head, not {q.dtype}, "
                           f"{heads}/{kv_heads} heads of {head_dim}")
@@ -1351,20 +1359,25 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         raise KernelError(f"the scale of the scores must be positive, got {scale}")
     if one_token_each and n_tokens != sequences:
         raise KernelError("one_token_each needs exactly one token per sequence")
-    if splits < 1 or splits > 65535:
-        raise KernelError(f"keys are cut into 1 to 65535 slices, not {splits}")
+    if not 0 <= splits <= 8:
+        raise KernelError(f"keys are cut into 1 to 8 slices, or into even runs (0), not {splits}")
     _need_aligned(q, "queries")
     _check_sinks(sinks, heads)
     _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
-    if splits > 8:
-        for t, count, name in ((part_acc, n_tokens * heads * splits * head_dim, "slice sums"), (part_ml, n_tokens * heads * splits * 2, "slice maxima")):
+    rows = 0
+    if splits == 0:
+        rows = attention_4bit_part_rows(q.device)
+        for t, count, name in ((part_acc, rows * head_dim, "part sums"), (part_ml, rows * 2, "part maxima")):
             if t is None or t.dtype != torch.float32 or t.numel() < count:
-                raise KernelError(f"attention_4bit: {splits} slices need {count} float32 {name}")
+                raise KernelError(f"attention_4bit: even runs need {count} float32 {name}")
+            _need_aligned(t, name)
+        if tickets is None or tickets.dtype != torch.int32 or tickets.numel() < 4 * sm_count(q.device):
+            raise KernelError(f"attention_4bit: even runs need {4 * sm_count(q.device)} int32 tickets")
     wide = not one_token_each and n_tokens > sequences                 # several tokens of a sequence share a pass over its keys
-    fn = _fn("cache_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppppp")
+    fn = _fn("attention_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppplppp")
     _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0], _ptr(cu), _ptr(len_before), sequences, n_tokens,
               heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, 1 if wide else 0, _ptr(out), _ptr(part_acc), _ptr(part_ml),
-              _ptr(status), _ptr(sinks), _stream()), "attention_4bit", 2 if splits > 8 else 1)
+              _ptr(tickets), rows, _ptr(status), _ptr(sinks), _stream()), "attention_4bit")
 
 
 # --------------------------------------------------------------------- latent attention

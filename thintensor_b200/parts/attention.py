@@ -338,6 +338,9 @@ class CausalAttention(Mixer):
 
     # ------------------------------------------------------------------ a cache in 4 bits
     EXPAND_4BIT_FROM = 16           # new tokens a sequence (on average) from which a step's blocks are expanded
+    # Keys times tiles from which few long tiles are cut into even runs instead of 8 slices (heads of 128, slices against runs: one sequence
+    # of 16,384 tokens, 8 heads, 18 and 22 us, of 32,768 29 and 27; four of 16,384 33 and 28; two of up to 40,001 42 and 33).
+    EVEN_4BIT_FROM = 8 * 24576
     EXPAND_4BIT_BYTES = 4 << 30     # most scratch memory that the expanded blocks may take
 
     def span_4bit(self, ctx, width: int) -> int:
@@ -372,14 +375,21 @@ class CausalAttention(Mixer):
                 api.attention_mma(q, keys, values, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
                                   self.head_dim, self.scale, self.reach, 1, mixed, None, None, ctx.status)
             return
-        # slices of the keys until the CTAs fill the GPU, each of 512 keys at least
-        tiles = ctx.sequences if ctx.decode else -(-ctx.n_tokens * (self.heads // self.kv_heads) // 16)
+        group, sms = self.heads // self.kv_heads, api.sm_count(ctx.status.device)
+        wide = group > 8 or ctx.n_tokens > ctx.sequences               # tiles of up to 16 rows, of which an SM holds half as many
+        units = (ctx.sequences if ctx.decode else -(-ctx.n_tokens * group // 16)) * self.kv_heads
         bound = min(ctx.max_total, self.window or self.chunk or ctx.max_total)
-        splits = max(1, min(api.sm_count(ctx.status.device) // max(1, tiles * self.kv_heads), bound // 512, 64))
-        part_acc, part_ml = self.slice_scratch(ctx, splits) if splits > 8 else (None, None)
+        part_acc = part_ml = tickets = None
+        if units * 8 <= 2 * sms and bound >= 8192 and bound * units >= self.EVEN_4BIT_FROM:
+            splits, rows = 0, api.attention_4bit_part_rows(ctx.status.device)
+            part_acc = ctx.scratch("attention.part_acc", (rows * self.head_dim,), torch.float32)
+            part_ml = ctx.scratch("attention.part_ml", (rows * 2,), torch.float32)
+            tickets = ctx.workspace.get_zeroed("attention.run_tickets", (4 * sms,), torch.int32)
+        else:       # slices of the keys until the CTAs fill the GPU once, each of 256 keys at least
+            splits = max(1, min((2 if wide else 4) * sms // max(1, units), bound // 256, 8))
         api.attention_4bit(q, cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
                            self.head_dim, self.scale, self.reach, splits, mixed, part_acc, part_ml, ctx.status, one_token_each=ctx.decode,
-                           sinks=self.sinks)
+                           sinks=self.sinks, tickets=tickets)
 
     TENSOR_CORES_FROM = 1           # packed tokens from which prompts run the tcgen05 kernel
 
