@@ -1906,6 +1906,55 @@ def sample_rows(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
               _ptr(request), _ptr(step), _ptr(out), _stream()), "sample_rows")
 
 
+def _row_setting(value, dtype: torch.dtype, rows: int, name: str, low: float | None = None, high: float | None = None) -> tuple:
+    """(pointer, number) of a setting that is a number for all rows or a tensor of one a row."""
+    if isinstance(value, torch.Tensor):
+        _need(value, dtype, name)
+        if value.numel() != rows:
+            raise KernelError(f"{name}: {rows} rows need as many numbers, got {value.numel()}")
+        return _ptr(value), 0
+    if not (value == value) or (low is not None and value < low) or (high is not None and value > high):
+        raise KernelError(f"{name} must lie between {low} and {high}, got {value}")
+    return 0, value
+
+
+def sample_filtered(logits: torch.Tensor, temperature, top_k, top_p, min_p, out: torch.Tensor, uniform: torch.Tensor | None = None, seed: int = 0,
+                    request: torch.Tensor | None = None, step: torch.Tensor | None = None) -> None:
+    """out[i] = a token drawn from float32 ``logits[i]`` [rows, vocab] with temperature, top-k, top-p and min-p, each a number or a tensor of
+    one a row (float32; ``top_k`` int32) on the device.  ``temperature`` 0: the largest logit, lowest id on ties; ``top_k`` 0, ``top_p`` 1 and
+    ``min_p`` 0 switch the filters off.  In this order: tokens below the k-th largest logit go (ties with it stay); then those for which
+    the probability of all strictly larger ones exceeds ``top_p``; then those whose probability is below ``min_p`` times the largest.
+    The token is the first in order of its id at which the rest's running probability exceeds ``uniform[i]`` (float32 in [0, 1)), or, without
+    ``uniform``, the number that :func:`sample_rows` takes for (``seed``, ``request[i]``, ``step[i]``).  NaN counts as minus infinity; a row
+    without anything above that gives token 0.  Tensors of settings are not looked at on the host: a negative or NaN temperature in one is
+    taken for 0, a ``min_p`` above 1 for 1."""
+    _need(out, torch.int32, "token output")
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise KernelError("logits must be float32 [rows, vocab] with their columns side by side")
+    rows, vocab = logits.shape
+    if out.numel() != rows:
+        raise KernelError(f"{rows} rows of logits give as many tokens, not {out.numel()}")
+    settings = (_row_setting(temperature, torch.float32, rows, "temperature", 0.0), _row_setting(top_k, torch.int32, rows, "top_k", 0, (1 << 31) - 1),
+                _row_setting(top_p, torch.float32, rows, "top_p", 0.0, 1.0), _row_setting(min_p, torch.float32, rows, "min_p", 0.0, 1.0))
+    if uniform is not None:
+        _need(uniform, torch.float32, "random numbers")
+        if uniform.numel() != rows:
+            raise KernelError(f"{rows} rows need as many random numbers, got {uniform.numel()}")
+    else:
+        for t, name in ((request, "request ids"), (step, "step ids")):
+            if t is None:
+                raise KernelError("sample_filtered needs random numbers, or request and step ids")
+            _need(t, torch.int32, name)
+            if t.numel() != rows:
+                raise KernelError(f"{rows} rows need as many {name}, got {t.numel()}")
+    if rows == 0:
+        return
+    fn = _fn("sampling_filters", "tt_sample_filtered", "pliipfpipfpfpupppp")
+    _check(fn(_ptr(logits), logits.stride(0), rows, vocab, settings[0][0], float(settings[0][1]), settings[1][0], int(settings[1][1]), settings[2][0],
+              float(settings[2][1]), settings[3][0], float(settings[3][1]), _ptr(uniform), seed & ((1 << 64) - 1), _ptr(request), _ptr(step), _ptr(out),
+              _stream()), "sample_filtered")
+
+
 # ----------------------------------------------------------------- tensor-core kernels
 _sm_counts: dict[int, int] = {}
 

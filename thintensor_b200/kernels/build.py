@@ -36,6 +36,7 @@ SOURCES: dict[str, list[str]] = {
     "gemm_simt": [],
     "gemm_split": [],
     "sampling": [],
+    "sampling_filters": [],
     "attention_static_scratch": [],
     "gemm_tcgen05": [],
     "attention_forms": [],
