@@ -20,6 +20,7 @@ _EXPORTS = {
     "DecoderModel": ("thintensor_b200.engine.model", "DecoderModel"),
     "run_generation": ("thintensor_b200.engine.generate", "run_generation"),
     "SamplingParams": ("thintensor_b200.sampling.sampler", "SamplingParams"),
+    "sample_given": ("thintensor_b200.sampling.sampler", "sample_given"),
     "SequenceCache": ("thintensor_b200.cache.cache", "SequenceCache"),
     "LlamaConfig": ("thintensor_b200.config.llama", "LlamaConfig"),
     "load_config": ("thintensor_b200.config.registry", "load_config"),

@@ -39,9 +39,11 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--temperature", type=float, default=0.0, help="Sampling temperature; 0 is greedy")
     run.add_argument("--top-p", type=float, default=1.0, help="Nucleus mass; 1 switches it off")
     run.add_argument("--top-k", type=int, default=0, help="Keep the k most likely tokens; 0 switches it off")
+    run.add_argument("--min-p", type=float, default=0.0, help="Drop tokens below this fraction of the likeliest one's probability; 0 switches it off")
     run.add_argument("--seed", type=int, default=0, help="Random seed")
     run.add_argument("--device", choices=["cuda"], default="cuda")
     run.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16")
+    run.add_argument("--cache", choices=["4bit"], help="Keep keys and values in 4 bits instead of --dtype")
     run.add_argument("--tokenizer", help="Tokenizer directory")
     run.add_argument("--batch-size", type=int, default=8, help="Most sequences decoded together")
     run.add_argument("--ignore-eos", action="store_true", help="Always generate --max-new-tokens tokens")
@@ -66,6 +68,7 @@ def build_parser() -> argparse.ArgumentParser:
     bench.add_argument("--seed", type=int, default=0)
     bench.add_argument("--device", choices=["cuda"], default="cuda")
     bench.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16")
+    bench.add_argument("--cache", choices=["4bit"], help="Keep keys and values in 4 bits instead of --dtype")
     bench.add_argument("--json", action="store_true")
     bench.add_argument("--out", help="Write JSON results to this file")
 
@@ -82,6 +85,7 @@ def build_parser() -> argparse.ArgumentParser:
     validate.add_argument("--seed", type=int, default=0)
     validate.add_argument("--device", choices=["cuda"], default="cuda")
     validate.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16")
+    validate.add_argument("--cache", choices=["4bit"], help="Keep keys and values in 4 bits instead of --dtype (the reference stays as it is)")
     validate.add_argument("--json", action="store_true")
 
     random = sub.add_parser("random", help="Write a model folder with random weights",
@@ -129,13 +133,15 @@ def cmd_run(args) -> int:
     if args.random_weights is not None:
         from thintensor_b200.config.base import read_config_json
 
-        runtime = thintensor_b200.random_model(read_config_json(args.model), seed=args.random_weights, dtype=args.dtype, device=args.device)
+        runtime = thintensor_b200.random_model(read_config_json(args.model), seed=args.random_weights, dtype=args.dtype, device=args.device,
+                                               cache=args.cache)
     else:
-        runtime = thintensor_b200.load_model(args.model, dtype=args.dtype, device=args.device)
+        runtime = thintensor_b200.load_model(args.model, dtype=args.dtype, device=args.device, cache=args.cache)
     started = time.perf_counter()
     outputs = runtime.generate(
         prompts, max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_p=args.top_p, top_k=args.top_k,
         seed=args.seed, stop_ids=() if args.ignore_eos else None, context=args.context, batch_size=args.batch_size,
+        min_p=args.min_p,
     )
     elapsed = time.perf_counter() - started
     new_tokens = sum(len(o) for o in outputs)
@@ -143,7 +149,8 @@ def cmd_run(args) -> int:
         print(json.dumps({
             "prompt_token_ids": prompts, "generated_token_ids": outputs, "new_tokens": new_tokens,
             "seconds": elapsed, "tokens_per_s": new_tokens / elapsed if elapsed > 0 else None,
-            "dtype": args.dtype, "temperature": args.temperature, "top_p": args.top_p, "top_k": args.top_k, "seed": args.seed,
+            "dtype": args.dtype, "temperature": args.temperature, "top_p": args.top_p, "top_k": args.top_k, "min_p": args.min_p, "seed": args.seed,
+            "cache": args.cache,
         }))
     else:
         for prompt, output in zip(prompts, outputs):
@@ -165,9 +172,9 @@ def cmd_bench(args) -> int:
         raise SystemExit("bench needs a model folder or --shape, not both")
     pk = peaks(args.peaks)
     if args.shape:
-        runtime = thintensor_b200.random_model(SHAPES[args.shape], seed=args.seed, dtype=args.dtype, device=args.device)
+        runtime = thintensor_b200.random_model(SHAPES[args.shape], seed=args.seed, dtype=args.dtype, device=args.device, cache=args.cache)
     else:
-        runtime = thintensor_b200.load_model(args.model, dtype=args.dtype, device=args.device)
+        runtime = thintensor_b200.load_model(args.model, dtype=args.dtype, device=args.device, cache=args.cache)
     batches = parse_ids(args.batch)
     if not batches or min(batches) <= 0:
         raise SystemExit("--batch must name positive numbers of sequences")
@@ -218,7 +225,7 @@ def cmd_bench(args) -> int:
         runs.append(run)
     first = runs[0]
     result = {
-        "model": str(args.model or args.shape), "dtype": args.dtype, "peaks": pk,
+        "model": str(args.model or args.shape), "dtype": args.dtype, "cache": args.cache, "peaks": pk,
         "batch_size": first["batch_size"], "prompt_tokens": first["prompt_tokens"], "steps": first["steps"],
         "warmup_steps": first["warmup_steps"], "context": first["context"],
         "tokens_per_s": first["tokens_per_s"], "ms_per_token": first["ms_per_step"],
@@ -247,10 +254,10 @@ def cmd_validate(args) -> int:
         with tempfile.TemporaryDirectory() as folder:      # both dtypes are read from the same file
             thintensor_b200.save_random_model(folder, SHAPES[args.shape], seed=args.seed, dtype="bfloat16")
             report = validate_model(folder, dtype=args.dtype, tokens=ids, length=args.length, seed=args.seed,
-                                    reference_logits=args.reference_logits, request=args.request)
+                                    reference_logits=args.reference_logits, request=args.request, cache=args.cache)
     else:
         report = validate_model(args.model, dtype=args.dtype, tokens=ids, length=args.length, seed=args.seed,
-                                reference_logits=args.reference_logits, request=args.request)
+                                reference_logits=args.reference_logits, request=args.request, cache=args.cache)
     print(json.dumps(report) if args.json else json.dumps(report, indent=2))
     order = {"fail": 0, "ranking_pass": 1, "exact_pass": 2}
     needed = {"ranking": 1, "exact": 2}[args.require_tier]

@@ -1906,6 +1906,9 @@ def sample_rows(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
               _ptr(request), _ptr(step), _ptr(out), _stream()), "sample_rows")
 
 
+SAMPLE_FILTERED_VOCAB = 8 * 65536
+
+
 def _row_setting(value, dtype: torch.dtype, rows: int, name: str, low: float | None = None, high: float | None = None) -> tuple:
     """(pointer, number) of a setting that is a number for all rows or a tensor of one a row."""
     if isinstance(value, torch.Tensor):
@@ -1932,6 +1935,8 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k, top_p, min_p, out:
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
         raise KernelError("logits must be float32 [rows, vocab] with their columns side by side")
     rows, vocab = logits.shape
+    if not 1 <= vocab <= SAMPLE_FILTERED_VOCAB:
+        raise KernelError(f"sample_filtered takes vocabularies of 1 to {SAMPLE_FILTERED_VOCAB} tokens, not {vocab}")
     if out.numel() != rows:
         raise KernelError(f"{rows} rows of logits give as many tokens, not {out.numel()}")
     settings = (_row_setting(temperature, torch.float32, rows, "temperature", 0.0), _row_setting(top_k, torch.int32, rows, "top_k", 0, (1 << 31) - 1),

@@ -109,7 +109,7 @@ class Runtime:
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 200, temperature: float = 0.0, top_p: float = 1.0,
                  top_k: int = 0, seed: int = 0, stop_ids: Sequence[int] | None = None, context: int | None = None,
-                 batch_size: int = 8, use_graph: bool = True, stats: GenerationStats | None = None) -> list[list[int]]:
+                 batch_size: int = 8, use_graph: bool = True, stats: GenerationStats | None = None, min_p: float = 0.0) -> list[list[int]]:
         """New tokens for every prompt (lists of token ids).  ``stop_ids`` default to the
         model's end-of-sequence ids; pass ``()`` to always generate ``max_new_tokens``."""
         prompts = [list(p) for p in prompts]
@@ -118,7 +118,7 @@ class Runtime:
         per_sequence = -(-longest // BLOCK_TOKENS) * BLOCK_TOKENS
         live = min(batch_size, max(1, len(prompts)))
         engine = self.engine_for(per_sequence * live, live)
-        backend = EngineBackend(engine, SamplingParams(temperature, top_k, top_p, seed), use_graph)
+        backend = EngineBackend(engine, SamplingParams(temperature, top_k, top_p, seed, min_p), use_graph)
         return run_generation(backend, prompts, max_new_tokens, stops, batch_size, context, stats)
 
 

@@ -159,11 +159,12 @@ def load_reference_logits(path, vocab: int, request: str | None = None):
     return tokens, positions, torch.stack([found[p] for p in positions])
 
 
-def validate_model(folder, dtype="bf16", tokens=None, length=96, seed=0, device="cuda", reference_logits=None, request=None) -> dict:
+def validate_model(folder, dtype="bf16", tokens=None, length=96, seed=0, device="cuda", reference_logits=None, request=None, cache=None) -> dict:
     """Run the three modes in ``dtype`` and compare them with ``reference_logits`` (a path, see
     :func:`load_reference_logits`) at the positions that file covers, or, without one, with this
-    engine's float32 path at every position."""
-    runtime = load_model(folder, dtype=dtype, device=device)
+    engine's float32 path at every position.  ``cache``: as for :func:`~thintensor_b200.runtime.load_model`, for the runtime
+    that is compared, never for the one it is compared with."""
+    runtime = load_model(folder, dtype=dtype, device=device, cache=cache)
     vocab = runtime.model.spec.vocab_size
     positions = None
     if reference_logits is not None:
@@ -177,7 +178,7 @@ def validate_model(folder, dtype="bf16", tokens=None, length=96, seed=0, device=
         g = torch.Generator().manual_seed(seed)
         tokens = torch.randint(0, vocab, (length,), generator=g).tolist()
     if reference_logits is None:
-        exact = runtime if dtype in ("fp32", "float32") else load_model(folder, dtype="fp32", device=device)
+        exact = runtime if dtype in ("fp32", "float32") and cache is None else load_model(folder, dtype="fp32", device=device)
         want = _whole(exact, tokens)
         against = "float32 engine, whole sequence (no outside reference given)"
     elif max(positions) >= len(tokens) or min(positions) < 0:
