@@ -89,7 +89,7 @@ struct Filter {
         const double base = sh->powers[n & 31];
         const double w = fma(base * r, s, base);
         const double scaled = __hiloint2double(__double2hiint(w) + (((n >> 5) + 45) << 20), __double2loint(w));
-        return x == top ? 35184372088832.0 : scaled;
+        return x == top ? 35184372088832.0 : x < far ? 0.0 : scaled;       // far is M itself where T is below its last bit
     }
     static __device__ __forceinline__ u64 units(double w) { return (u64)__double_as_longlong(w + 6755399441055744.0) - 0x4338000000000000ull; }
     __device__ __forceinline__ u64 mass(float x) const { return units(weight(x)); }
