@@ -44,145 +44,64 @@ __device__ __forceinline__ Group4 group_of_lanes(const float (&x)[4]) {
     return group_of(least, greatest, bad);
 }
 
-// four neighbouring numbers, summed over the k-slices of the projection
+// four neighbouring numbers of one k-slice of the projection
 template <bool VEC>
-__device__ __forceinline__ void load_sums(const float* __restrict__ p, int splits, size_t stride, float (&x)[4]) {
-    x[0] = x[1] = x[2] = x[3] = 0.0f;
-    for (int s = 0; s < splits; ++s, p += stride) {
-        if (VEC) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-            x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
-        } else {
+__device__ __forceinline__ void load_four(const float* __restrict__ p, float (&x)[4]) {
+    if (VEC) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] += __ldg(p + k);
-        }
+        for (int k = 0; k < 4; ++k) x[k] = __ldg(p + k);
     }
 }
 
-constexpr int APPEND_WARPS = 4;
+constexpr int APPEND_WARPS = 8;
 constexpr int APPEND_MAX_HALF = 64;
 
-// A warp takes rows (a head of a token) with four numbers a lane: queries and keys are rotated, queries narrowed, keys quantised;
-// a row of values stands for up to four tokens of the sequence, those that share its code words with the token that owns them (the
-// first of the step among them).  The angle position * frequency is formed in float64 and brought into one turn before the sine and
-// cosine are taken in float32: a float32 product of a position in the hundred thousands is off by a hundredth of a radian, which moves
-// codes.  grid = (tokens, parts).
-template <int D, bool VEC>
-__global__ void __launch_bounds__(APPEND_WARPS * 32)
-rope_append_4bit_kernel(const float* __restrict__ qkv, int splits, size_t split_stride, const float* __restrict__ inv_freq, int rotary_dim,
-                        int interleaved, float attention_scaling, __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_pool,
-                        uint8_t* __restrict__ v_pool, const int* __restrict__ table, int table_width, int pool_blocks,
-                        const int* __restrict__ cu, const int* __restrict__ len_before, int sequences, int heads, int kv_heads,
-                        int write_cache, unsigned* status) {
-    constexpr int G = D / 32, LANES = D / 4, ROWS = 32 / LANES;        // lanes of a row, rows of a warp
-    // Dependents start only behind this wait: a kernel that reads cache blocks ahead of its own wait then meets nothing older than this
-    // launch still on its way.
-    tt_pdl_wait();
-    tt_pdl_launch_dependents();
-    const int t = blockIdx.x;
-    const int b = (sequences == (int)gridDim.x && cu[t] == t && cu[t + 1] == t + 1) ? t : tt_find_sequence(cu, sequences, t);
-    const int seq_end = cu[b + 1];
-    if (t >= seq_end) return;                                          // a row behind the last sequence
-    const int pos = len_before[b] + (t - cu[b]);
-    const int half = rotary_dim >> 1;
-    __shared__ float cos_sh[APPEND_MAX_HALF], sin_sh[APPEND_MAX_HALF];
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        const double angle = (double)__ldg(inv_freq + i) * (double)pos;
-        const double turned = fma(-rint(angle * 0.15915494309189535), 6.283185307179586, angle);
-        float si, co;
-        sincosf((float)turned, &si, &co);
-        cos_sh[i] = co * attention_scaling;
-        sin_sh[i] = si * attention_scaling;
-    }
-    int block = -1;
-    if (write_cache) {
-        const int entry = pos / TT_BLOCK_TOKENS;
-        block = entry < table_width ? table[(size_t)b * table_width + entry] : -1;
-        if (block >= pool_blocks) block = -1;
-        if (block < 0 && threadIdx.x == 0) atomicOr(status, TT_STATUS_BAD_BLOCK);
-    }
-    const int slot = pos % TT_BLOCK_TOKENS;
-    __syncthreads();
-    const int cols = (heads + (write_cache ? 2 * kv_heads : 0)) * D;
-    const float* row = qkv + (size_t)t * cols;
+// The values of a CTA's tokens: a warp takes a head of the (up to) four tokens that an owner among them stands for.
+template <int D, bool VEC, int TOKENS>
+__device__ __forceinline__ void values_of_tokens(const float* __restrict__ qkv, int splits, size_t split_stride, uint8_t* __restrict__ v_pool, int t0, int cols,
+                                                 int rot_heads, int kv_heads, const int* pos_sh, const int* block_sh, const int* left_sh, const int* first_sh) {
+    constexpr int G = D / 32, LANES = D / 4, ROWS = 32 / LANES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES;
-    const int d0 = 4 * l, g = l >> 3, j = l & 7;
-    const int rot_heads = heads + (write_cache ? kv_heads : 0);
-    const int n_rot = (rot_heads + ROWS - 1) / ROWS;
-    const bool owner = write_cache && block >= 0 && ((pos & 3) == 0 || t == cu[b]);
-    const int n_val = owner ? (kv_heads + ROWS - 1) / ROWS : 0;
-    for (int item = blockIdx.y * APPEND_WARPS + warp; item < n_rot + n_val; item += gridDim.y * APPEND_WARPS) {
-        if (item < n_rot) {
-            const int head = item * ROWS + sub;
-            const bool active = sub < ROWS && head < rot_heads;
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4];
-            const float* p = row + (size_t)head * D;
-            if (active) load_sums<VEC>(p + d0, splits, split_stride, x);
-            if (interleaved) {
-#pragma unroll
-                for (int k = 0; k < 4; k += 2) {
-                    const int i = (d0 + k) >> 1;
-                    const bool turn = d0 + k < rotary_dim;
-                    const float co = turn ? cos_sh[i] : 1.0f, si = turn ? sin_sh[i] : 0.0f;
-                    y[k] = turn ? __fsub_rn(__fmul_rn(x[k], co), __fmul_rn(x[k + 1], si)) : x[k];
-                    y[k + 1] = turn ? __fadd_rn(__fmul_rn(x[k + 1], co), __fmul_rn(x[k], si)) : x[k + 1];
-                }
-            } else {
-                float other[4];                                        // the numbers that these are paired with
-                if (VEC) {                                             // half a multiple of four: they are another lane's four
-                    const int from = sub * LANES + (d0 < half ? l + (half >> 2) : (d0 < rotary_dim ? l - (half >> 2) : l));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) other[k] = __shfl_sync(0xffffffffu, x[k], from);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int d = d0 + k;
-                        other[k] = 0.0f;
-                        if (active && d < rotary_dim)
-                            for (int s = 0; s < splits; ++s) other[k] += __ldg(p + (d < half ? d + half : d - half) + s * split_stride);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int d = d0 + k;
-                    if (d < half) y[k] = __fsub_rn(__fmul_rn(x[k], cos_sh[d]), __fmul_rn(other[k], sin_sh[d]));
-                    else if (d < rotary_dim) y[k] = __fadd_rn(__fmul_rn(x[k], cos_sh[d - half]), __fmul_rn(other[k], sin_sh[d - half]));
-                    else y[k] = x[k];
-                }
-            }
-            if (active && head < heads) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
-                uint2 v;
-                v.x = *reinterpret_cast<const uint32_t*>(&lo);
-                v.y = *reinterpret_cast<const uint32_t*>(&hi);
-                *reinterpret_cast<uint2*>(q_out + ((size_t)t * heads + head) * D + d0) = v;
-            }
-            if (item * ROWS + ROWS <= heads) continue;                 // queries alone (the same for the whole warp)
-            const Group4 grp = group_of_lanes(y);
-            const int at = 8 * (j & 1);
-            uint32_t word = code_of(grp, y[0]) << at | code_of(grp, y[1]) << (at + 16) | code_of(grp, y[2]) << (at + 4) | code_of(grp, y[3]) << (at + 20);
-            word |= __shfl_xor_sync(0xffffffffu, word, 1);
-            if (active && head >= heads && block >= 0) {
-                uint8_t* dst = k_pool + ((size_t)block * kv_heads + (head - heads)) * block_bytes(D);
-                if (!(j & 1)) reinterpret_cast<uint32_t*>(dst)[(slot * 4 + (j >> 1)) * G + g] = word;
-                if (j == 0) reinterpret_cast<uint32_t*>(dst + code_bytes(D))[slot * G + g] = scale_bits(grp) | least_bits(grp) << 16;
-            }
-            continue;
-        }
-        const int kh = (item - n_rot) * ROWS + sub;
+    const int d0 = 4 * l, g = l >> 3, j = l & 7, n_val = (kv_heads + ROWS - 1) / ROWS;
+    // from the last warps on, which have the fewest rows of queries and keys
+    for (int item = gridDim.y * APPEND_WARPS - 1 - (int)(blockIdx.y * APPEND_WARPS + warp); item < TOKENS * n_val; item += gridDim.y * APPEND_WARPS) {
+        const int tok = item / n_val, t = t0 + tok, pos = pos_sh[tok], block = block_sh[tok], slot = pos % TT_BLOCK_TOKENS;
+        if (block < 0 || left_sh[tok] <= 0 || ((pos & 3) != 0 && !first_sh[tok])) continue;    // another token owns the words (the same for the whole warp)
+        const int kh = item % n_val * ROWS + sub;
         const bool active = sub < ROWS && kh < kv_heads;
         uint8_t* dst = v_pool + ((size_t)block * kv_heads + (active ? kh : 0)) * block_bytes(D);
         uint16_t* scales = reinterpret_cast<uint16_t*>(dst + code_bytes(D));
-        const int first = pos & 3, last = min(3, first + seq_end - 1 - t);   // the step's tokens among the word's four
+        const int first = pos & 3, last = min(3, first + left_sh[tok] - 1);    // the step's tokens among the words' four
+        const float* row = qkv + (size_t)t * cols + (size_t)(rot_heads + (active ? kh : 0)) * D + d0;
+        float v[4][4];
+        for (int s = 0; s < splits; ++s) {
+            float more[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                more[q][0] = more[q][1] = more[q][2] = more[q][3] = 0.0f;
+                if (active && q >= first && q <= last) load_four<VEC>(row + (ptrdiff_t)(q - first) * cols + s * split_stride, more[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[q][k] = s ? v[q][k] + more[q][k] : more[q][k];
+        }
+        const int a = slot >> 4, c = (slot >> 2) & 3, pick = j & 2;
+        uint32_t* to = reinterpret_cast<uint32_t*>(dst) + ((((a * G + g) * 8 + 4 * (j & 1) + pick) * 4 + c) * 2 + (j >> 2));
+        uint32_t old0 = 0u, old1 = 0u;
+        if (active && first != 0) { old0 = to[0]; old1 = to[8]; }      // older tokens' codes stay
         uint32_t words[4] = {0u, 0u, 0u, 0u}, fresh = 0u;
-        for (int q = first; q <= last; ++q) {
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (active) load_sums<VEC>(row + (size_t)(q - first) * cols + (size_t)(rot_heads + kh) * D + d0, splits, split_stride, x);
-            const Group4 grp = group_of_lanes(x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (q < first || q > last) continue;
+            const Group4 grp = group_of_lanes(v[q]);
             const int at = 8 * (q >> 1) + 16 * (q & 1);
             fresh |= 0xffu << at;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) words[k] |= code_of(grp, x[k]) << (at + 4 * ((j >> 1) & 1));
+            for (int k = 0; k < 4; ++k) words[k] |= code_of(grp, v[q][k]) << (at + 4 * ((j >> 1) & 1));
             if (active && j == 0) {
                 const int token = (slot & ~3) + q;
                 scales[token * G + g] = (uint16_t)scale_bits(grp);
@@ -192,34 +111,180 @@ rope_append_4bit_kernel(const float* __restrict__ qkv, int splits, size_t split_
 #pragma unroll
         for (int k = 0; k < 4; ++k) words[k] |= __shfl_xor_sync(0xffffffffu, words[k], 2);      // numbers r and r + 8 share a word
         if (active) {
-            const int a = slot >> 4, c = (slot >> 2) & 3, pick = j & 2;
-            uint32_t* to = reinterpret_cast<uint32_t*>(dst) + ((((a * G + g) * 8 + 4 * (j & 1) + pick) * 4 + c) * 2 + (j >> 2));
-            const uint32_t w0 = pick ? words[2] : words[0], w1 = pick ? words[3] : words[1];
-            if (first == 0) {                                          // nothing older in these words
-                to[0] = w0;
-                to[8] = w1;
-            } else {
-                to[0] = (to[0] & ~fresh) | w0;
-                to[8] = (to[8] & ~fresh) | w1;
-            }
+            to[0] = (old0 & ~fresh) | (pick ? words[2] : words[0]);
+            to[8] = (old1 & ~fresh) | (pick ? words[3] : words[1]);
         }
     }
+}
+
+// A warp takes rows (a head of a token) with four numbers a lane: queries and keys are rotated, queries narrowed, keys quantised;
+// a row of values stands for up to four tokens of the sequence, those that share its code words with the token that owns them (the
+// first of the step among them).  The angle position * frequency is formed in float64 and brought into one turn before the sine and
+// cosine are taken in float32: a float32 product of a position in the hundred thousands is off by a hundredth of a radian, which moves
+// codes.
+//
+// Prompts: a CTA takes TOKENS = 4 neighbouring tokens, whose places are looked up and whose 4 x 64 sines are taken by all its threads at
+// once; a warp's rows are one token's, two at a time, and the next two are asked for before it works on them (2,048 tokens of 32/8 heads of 128: 21
+// us, of which the bytes take 10; bound by the instructions of a row of keys or values, a hundred and more).  Few tokens: one a CTA, and as many
+// CTAs a token as give every warp a row (8 tokens of 32/8 heads of 64 in four slices: 4 us).  grid = (tokens / TOKENS, parts).
+template <int D, bool VEC, int TOKENS>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, TOKENS == 1 ? 2 : 4)
+rope_append_4bit_kernel(const float* __restrict__ qkv, int splits, size_t split_stride, const float* __restrict__ inv_freq, int rotary_dim,
+                        int interleaved, float attention_scaling, __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_pool,
+                        uint8_t* __restrict__ v_pool, const int* __restrict__ table, int table_width, int pool_blocks,
+                        const int* __restrict__ cu, const int* __restrict__ len_before, int sequences, int n_tokens, int heads, int kv_heads,
+                        int write_cache, unsigned* status) {
+    constexpr int G = D / 32, LANES = D / 4, ROWS = 32 / LANES;        // lanes of a row, rows of a warp
+    __shared__ float cos_sh[TOKENS][APPEND_MAX_HALF], sin_sh[TOKENS][APPEND_MAX_HALF];
+    __shared__ int pos_sh[TOKENS], block_sh[TOKENS], left_sh[TOKENS], first_sh[TOKENS];        // left: tokens of the sequence from this one on, 0: none of any
+    // Dependents start only behind this wait: a kernel that reads cache blocks ahead of its own wait then meets nothing older than this
+    // launch still on its way.
+    tt_pdl_wait();
+    tt_pdl_launch_dependents();
+    const int t0 = blockIdx.x * TOKENS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES;
+    const int d0 = 4 * l, g = l >> 3, j = l & 7;
+    const int rot_heads = heads + (write_cache ? kv_heads : 0);
+    const int n_rot = (rot_heads + ROWS - 1) / ROWS;
+    const int cols = (heads + (write_cache ? 2 * kv_heads : 0)) * D;
+    // a warp's rows belong to one token: rows first_row, first_row + step, ... of its queries and keys, APPEND_ROWS at a time
+    constexpr int PER_TOKEN = APPEND_WARPS / TOKENS, APPEND_ROWS = TOKENS == 1 ? 1 : 2, SLICES = TOKENS == 1 ? 3 : 1;
+    const int tok = warp / PER_TOKEN, t = t0 + tok, step = gridDim.y * PER_TOKEN;
+    int at_row = blockIdx.y * PER_TOKEN + warp % PER_TOKEN;
+    const float* token_row = qkv + (size_t)t * cols + d0;
+    auto mine = [&](int row) { return t < n_tokens && sub < ROWS && row * ROWS + sub < rot_heads; };
+    // Slice s of the rows from `from` on, without touching what comes back: a thread waits for a number where it first computes with it.
+    auto ask = [&](int from, int s, float (&x)[APPEND_ROWS][4]) {
+#pragma unroll
+        for (int i = 0; i < APPEND_ROWS; ++i) {
+            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+            if (mine(from + i * step)) load_four<VEC>(token_row + (size_t)((from + i * step) * ROWS + sub) * D + s * split_stride, x[i]);
+        }
+    };
+    float x[APPEND_ROWS][4];
+    ask(at_row, 0, x);                                                 // on their way while the places are looked up
+    if (threadIdx.x < TOKENS) {
+        const int u = t0 + threadIdx.x;
+        int left = 0, pos = 0, block = -1, first = 0;
+        if (u < n_tokens) {
+            const int b = (TOKENS == 1 && sequences == (int)gridDim.x && cu[u] == u && cu[u + 1] == u + 1) ? u : tt_find_sequence(cu, sequences, u);
+            left = max(0, cu[b + 1] - u);                              // a row behind the last sequence has none
+            first = u == cu[b];
+            pos = len_before[b] + (u - cu[b]);
+            if (write_cache && left > 0) {
+                const int entry = pos / TT_BLOCK_TOKENS;
+                block = entry < table_width ? table[(size_t)b * table_width + entry] : -1;
+                if (block >= pool_blocks) block = -1;
+                if (block < 0) { block = -1; atomicOr(status, TT_STATUS_BAD_BLOCK); }
+            }
+        }
+        pos_sh[threadIdx.x] = pos; block_sh[threadIdx.x] = block; left_sh[threadIdx.x] = left; first_sh[threadIdx.x] = first;
+    }
+    __syncthreads();
+    const int half = rotary_dim >> 1;
+    for (int i = threadIdx.x; i < TOKENS * half; i += APPEND_WARPS * 32) {
+        const int of = i / half, f = i - of * half;
+        const double angle = (double)__ldg(inv_freq + f) * (double)pos_sh[of];
+        const double turned = fma(-rint(angle * 0.15915494309189535), 6.283185307179586, angle);
+        float si, co;
+        sincosf((float)turned, &si, &co);
+        cos_sh[of][f] = co * attention_scaling;
+        sin_sh[of][f] = si * attention_scaling;
+    }
+    __syncthreads();
+    // the sines of this lane's four numbers: y = x * co + partner * si
+    float co[4], si[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int d = d0 + k, f = interleaved ? d >> 1 : (d < half ? d : d - half);
+        const bool turn = d < rotary_dim;
+        co[k] = turn ? cos_sh[tok][f] : 1.0f;
+        si[k] = turn ? sin_sh[tok][f] : 0.0f;
+        if (interleaved ? !(d & 1) : d < half) si[k] = -si[k];
+    }
+    const int from_lane = sub * LANES + (d0 < half ? l + (half >> 2) : (d0 < rotary_dim ? l - (half >> 2) : l));
+    const bool there = left_sh[tok] > 0;
+    const int block = block_sh[tok], slot = pos_sh[tok] % TT_BLOCK_TOKENS;
+    for (; at_row < n_rot; at_row += APPEND_ROWS * step) {
+        for (int s = 1; s < splits; s += SLICES) {
+            float more[SLICES][APPEND_ROWS][4];
+#pragma unroll
+            for (int e = 0; e < SLICES; ++e)
+                if (s + e < splits) ask(at_row, s + e, more[e]);
+#pragma unroll
+            for (int e = 0; e < SLICES; ++e)
+#pragma unroll
+                for (int i = 0; i < APPEND_ROWS; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (s + e < splits) x[i][k] += more[e][i][k];
+        }
+        float ahead[APPEND_ROWS][4];
+        ask(at_row + APPEND_ROWS * step, 0, ahead);
+#pragma unroll
+        for (int i = 0; i < APPEND_ROWS; ++i) {
+            const int row = at_row + i * step;                         // the same for the whole warp
+            if (row >= n_rot) break;
+            const int head = row * ROWS + sub;
+            const bool active = there && sub < ROWS && head < rot_heads;
+            float y[4], other[4];                                      // the numbers that these are paired with
+            if (interleaved) {
+                other[0] = x[i][1]; other[1] = x[i][0]; other[2] = x[i][3]; other[3] = x[i][2];
+            } else if (VEC) {                                          // half a multiple of four: they are another lane's four
+#pragma unroll
+                for (int k = 0; k < 4; ++k) other[k] = __shfl_sync(0xffffffffu, x[i][k], from_lane);
+            } else {
+                const float* p = token_row - d0 + (size_t)head * D;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int d = d0 + k;
+                    other[k] = 0.0f;
+                    if (active && d < rotary_dim)
+                        for (int s = 0; s < splits; ++s) other[k] += __ldg(p + (d < half ? d + half : d - half) + s * split_stride);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = d0 + k < rotary_dim ? __fadd_rn(__fmul_rn(x[i][k], co[k]), __fmul_rn(other[k], si[k])) : x[i][k];
+            if (active && head < heads) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
+                uint2 v;
+                v.x = *reinterpret_cast<const uint32_t*>(&lo);
+                v.y = *reinterpret_cast<const uint32_t*>(&hi);
+                *reinterpret_cast<uint2*>(q_out + ((size_t)t * heads + head) * D + d0) = v;
+            }
+            if (row * ROWS + ROWS <= heads) continue;                  // queries alone
+            const Group4 grp = group_of_lanes(y);
+            const int at = 8 * (j & 1);
+            uint32_t word = code_of(grp, y[0]) << at | code_of(grp, y[1]) << (at + 16) | code_of(grp, y[2]) << (at + 4) | code_of(grp, y[3]) << (at + 20);
+            word |= __shfl_xor_sync(0xffffffffu, word, 1);
+            if (active && head >= heads && block >= 0) {
+                uint8_t* dst = k_pool + ((size_t)block * kv_heads + (head - heads)) * block_bytes(D);
+                if (!(j & 1)) reinterpret_cast<uint32_t*>(dst)[(slot * 4 + (j >> 1)) * G + g] = word;
+                if (j == 0) reinterpret_cast<uint32_t*>(dst + code_bytes(D))[slot * G + g] = scale_bits(grp) | least_bits(grp) << 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < APPEND_ROWS; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[i][k] = ahead[i][k];
+    }
+    if (write_cache) values_of_tokens<D, VEC, TOKENS>(qkv, splits, split_stride, v_pool, t0, cols, rot_heads, kv_heads, pos_sh, block_sh, left_sh, first_sh);
 }
 
 // ---------------------------------------------------------------------------------------------------------- reading back
 // The blocks that a step sees, as bfloat16 blocks like the plain cache's (keys [token][D], values [D][token]), for kernels that read
 // those: block w of sequence b goes to place b * span + w - (its first block that is seen), and table_tmp names the places (-1: not
 // seen, or outside the pool).  Tokens behind the sequence's end become zeros.  Bound by the 16 bits a number that it writes.
-// grid = (span, kv_heads, sequences).
+// grid = (2 * span, kv_heads, sequences): keys and values are CTAs of their own.
 template <int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, const int* __restrict__ table, int table_width,
                    int pool_blocks, const int* __restrict__ cu, const int* __restrict__ len_before, int kv_heads, int window, int span,
                    __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values, int* __restrict__ table_tmp, unsigned* status) {
     constexpr int G = D / 32;
     tt_pdl_wait();
     tt_pdl_launch_dependents();
-    const int b = blockIdx.z, kh = blockIdx.y;
+    const int b = blockIdx.z, kh = blockIdx.y, place = blockIdx.x >> 1;
     const int before = len_before[b], length = before + cu[b + 1] - cu[b];
     const int first = tt_first_key(before, window) / TT_BLOCK_TOKENS, last = length > before ? (length - 1) / TT_BLOCK_TOKENS : first - 1;
     const int* table_row = table + (size_t)b * table_width;
@@ -230,7 +295,7 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
         }
         if (threadIdx.x == 0 && last - first >= span) atomicOr(status, TT_STATUS_BAD_SHAPE);
     }
-    const int w = first + blockIdx.x;
+    const int w = first + place;
     if (w > last) return;
     const int block = w < table_width ? table_row[w] : -1;
     if (block < 0 || block >= pool_blocks) {
@@ -238,38 +303,38 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
         return;
     }
     const int left = length - w * TT_BLOCK_TOKENS;                     // tokens of this block
-    const size_t from = ((size_t)block * kv_heads + kh) * block_bytes(D), to = ((size_t)(b * span + blockIdx.x) * kv_heads + kh) * TT_BLOCK_TOKENS * D;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pool + from);
-    const uint32_t* pairs = words + code_bytes(D) / 4;
-    for (int i = threadIdx.x; i < TT_BLOCK_TOKENS * 4 * G; i += blockDim.x) {
-        const int c = i & 3, g = (i >> 2) % G, token = (i >> 2) / G;   // eight neighbouring numbers
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (token < left) {
+    const size_t from = ((size_t)block * kv_heads + kh) * block_bytes(D), to = ((size_t)(b * span + place) * kv_heads + kh) * TT_BLOCK_TOKENS * D;
+    if (!(blockIdx.x & 1)) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pool + from);
+        const uint32_t* pairs = words + code_bytes(D) / 4;
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            const int i = k * 256 + threadIdx.x;
+            const int c = i & 3, g = (i >> 2) % G, token = (i >> 2) / G;       // eight neighbouring numbers
             const uint32_t word = __ldg(words + (token * 4 + c) * G + g), pair = __ldg(pairs + token * G + g);
             const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
             uint32_t out[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const __nv_bfloat162 two = __floats2bfloat162_rn(fmaf(s, (float)((word >> (4 * k)) & 15u), m), fmaf(s, (float)((word >> (4 * k + 16)) & 15u), m));
-                out[k] = *reinterpret_cast<const uint32_t*>(&two);
+            for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(fmaf(s, (float)((word >> (4 * e)) & 15u), m), fmaf(s, (float)((word >> (4 * e + 16)) & 15u), m));
+                out[e] = token < left ? *reinterpret_cast<const uint32_t*>(&two) : 0u;
             }
-            v = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(keys + to + (size_t)token * D + 32 * g + 8 * c) = make_uint4(out[0], out[1], out[2], out[3]);
         }
-        *reinterpret_cast<uint4*>(keys + to + (size_t)token * D + 32 * g + 8 * c) = v;
+        return;
     }
-    words = reinterpret_cast<const uint32_t*>(v_pool + from);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + from);
     const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(words + code_bytes(D) / 4);
     const __nv_bfloat16* least = scales + TT_BLOCK_TOKENS * G;
-    for (int i = threadIdx.x; i < 16 * 16 * G; i += blockDim.x) {      // four tokens of two numbers
-        const int c = i & 3, a = (i >> 2) & 3, r = (i >> 4) & 7, jj = (i >> 7) & 1, g = i >> 8;
-        const uint32_t word = __ldg(words + (((a * G + g) * 8 + r) * 4 + c) * 2 + jj);
-        const int token = 16 * a + 4 * c;
-        float s[4], m[4];
+    const int c = threadIdx.x & 3, a = (threadIdx.x >> 2) & 3, r = (threadIdx.x >> 4) & 7, jj = threadIdx.x >> 7, token = 16 * a + 4 * c;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            s[k] = __bfloat162float(scales[(token + k) * G + g]);
-            m[k] = __bfloat162float(least[g * TT_BLOCK_TOKENS + token + k]);
-        }
+    for (int g = 0; g < G; ++g) {                                      // four tokens of two numbers
+        const uint32_t word = __ldg(words + (((a * G + g) * 8 + r) * 4 + c) * 2 + jj);
+        const uint2 low = __ldg(reinterpret_cast<const uint2*>(least + g * TT_BLOCK_TOKENS + token));
+        const float m[4] = {__uint_as_float(low.x << 16), __uint_as_float(low.x & 0xffff0000u), __uint_as_float(low.y << 16), __uint_as_float(low.y & 0xffff0000u)};
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = __bfloat162float(scales[(token + k) * G + g]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float x[4];
@@ -298,13 +363,13 @@ extern "C" int tt_rope_append_4bit(const float* qkv, int splits, long long split
     const bool vec = rotary_dim % 8 == 0 && split_stride % 4 == 0 && ((uintptr_t)qkv & 15) == 0;
     const int rows_per_warp = 32 / (head_dim / 4);
     const int items = (heads + (write_cache ? kv_heads : 0) + rows_per_warp - 1) / rows_per_warp + (write_cache ? (kv_heads + rows_per_warp - 1) / rows_per_warp : 0);
-    // few tokens: a row a warp; prompts: a CTA a token, whose sines are taken once
-    const int parts = n_tokens >= 512 ? 1 : (items + APPEND_WARPS - 1) / APPEND_WARPS;
-#define TT_LAUNCH(D, V)                                                                                                                               \
-    tt_launch_pdl(rope_append_4bit_kernel<D, V>, dim3(n_tokens, parts), dim3(APPEND_WARPS * 32), 0, stream, qkv, splits, (size_t)split_stride, inv_freq, \
-                  rotary_dim, interleaved, attention_scaling, (__nv_bfloat16*)q_out, (uint8_t*)k_pool, (uint8_t*)v_pool, table, table_width, pool_blocks, \
-                  cu, len_before, sequences, heads, kv_heads, write_cache, status)
-#define TT_LAUNCH_D(D) (vec ? TT_LAUNCH(D, true) : TT_LAUNCH(D, false))
+    const bool many = n_tokens >= 256;                                  // (598 tokens of 20/4 heads of 96: 18 us with a token a CTA, 10 with four)
+    const dim3 grid(many ? (n_tokens + 3) / 4 : n_tokens, many ? 1 : (items + APPEND_WARPS - 1) / APPEND_WARPS);
+#define TT_LAUNCH(D, V, T)                                                                                                                            \
+    tt_launch_pdl(rope_append_4bit_kernel<D, V, T>, grid, dim3(APPEND_WARPS * 32), 0, stream, qkv, splits, (size_t)split_stride, inv_freq, rotary_dim, \
+                  interleaved, attention_scaling, (__nv_bfloat16*)q_out, (uint8_t*)k_pool, (uint8_t*)v_pool, table, table_width, pool_blocks, cu,     \
+                  len_before, sequences, n_tokens, heads, kv_heads, write_cache, status)
+#define TT_LAUNCH_D(D) (vec ? (many ? TT_LAUNCH(D, true, 4) : TT_LAUNCH(D, true, 1)) : (many ? TT_LAUNCH(D, false, 4) : TT_LAUNCH(D, false, 1)))
     switch (head_dim) {
         case 32: TT_LAUNCH_D(32); break;
         case 64: TT_LAUNCH_D(64); break;
@@ -321,9 +386,10 @@ extern "C" int tt_expand_4bit(const void* k_pool, const void* v_pool, const int*
                               int* table_tmp, unsigned* status, cudaStream_t stream) {
     if (sequences <= 0) return 0;
     if (!cache4::takes(kv_heads, kv_heads, head_dim) || span < 1 || sequences > 65535 || (((uintptr_t)keys | (uintptr_t)values) & 15) != 0) return (int)cudaErrorInvalidValue;
-    const dim3 grid(span, kv_heads, sequences);
+    if (span > (1 << 29)) return (int)cudaErrorInvalidValue;
+    const dim3 grid(2 * span, kv_heads, sequences);
 #define TT_LAUNCH(D)                                                                                                                             \
-    tt_launch_pdl(expand_4bit_kernel<D>, grid, dim3(128), 0, stream, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, \
+    tt_launch_pdl(expand_4bit_kernel<D>, grid, dim3(256), 0, stream, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, \
                   cu, len_before, kv_heads, window, span, (__nv_bfloat16*)keys, (__nv_bfloat16*)values, table_tmp, status)
     switch (head_dim) {
         case 32: TT_LAUNCH(32); break;

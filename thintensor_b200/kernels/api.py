@@ -1254,23 +1254,29 @@ def cache_4bit_bytes(head_dim: int) -> int:
 
 
 def _check_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
-                kv_heads: int, head_dim: int, status: torch.Tensor) -> None:
-    for t, name in ((k_pool, "the 4-bit key pool"), (v_pool, "the 4-bit value pool")):
-        _need(t, torch.uint8, name)
-        if t.dim() != 3 or tuple(t.shape[1:]) != (kv_heads, cache_4bit_bytes(head_dim)):
-            raise KernelError(f"{name} must be [blocks, {kv_heads}, {cache_4bit_bytes(head_dim)}] bytes, got {tuple(t.shape)}")
-        _need_aligned(t, name)
-    if k_pool.shape[0] != v_pool.shape[0]:
-        raise KernelError("the 4-bit pools must have as many blocks of values as of keys")
-    _check_step(table, cu, len_before, sequences, status)
+                kv_heads: int, head_dim: int, status: torch.Tensor) -> tuple[int, int]:
+    """Checks a step over a cache in 4 bits; returns the table's width and the pools' blocks."""
+    _need(k_pool, torch.uint8, "the 4-bit key pool")
+    _need(v_pool, torch.uint8, "the 4-bit value pool")
+    shape = k_pool.shape
+    if v_pool.shape != shape or len(shape) != 3 or shape[1] != kv_heads or shape[2] != 40 * head_dim:
+        raise KernelError(f"the 4-bit pools must be alike, with as many blocks of values as of keys, [blocks, {kv_heads}, {cache_4bit_bytes(head_dim)}] bytes; got "
+                          f"{tuple(shape)} and {tuple(v_pool.shape)}")
+    if k_pool.data_ptr() % 16 or v_pool.data_ptr() % 16:
+        raise KernelError("the 4-bit pools must start on a 16-byte boundary")
+    return _check_step(table, cu, len_before, sequences, status), shape[0]
 
 
-def _check_step(table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int, status: torch.Tensor) -> None:
-    for t, name in ((table, "the block table"), (cu, "token offsets"), (len_before, "lengths"), (status, "the status word")):
-        _need(t, torch.int32, name)
-    if sequences < 1 or table.dim() != 2 or table.shape[0] < sequences or cu.numel() < sequences + 1 or len_before.numel() < sequences:
+def _check_step(table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int, status: torch.Tensor) -> int:
+    _need(table, torch.int32, "the block table")
+    _need(cu, torch.int32, "token offsets")
+    _need(len_before, torch.int32, "lengths")
+    _need(status, torch.int32, "the status word")
+    shape = table.shape
+    if sequences < 1 or len(shape) != 2 or shape[0] < sequences or cu.numel() <= sequences or len_before.numel() < sequences:
         raise KernelError(f"a step of {sequences} sequences needs a table row and a length for each and one offset more, got "
-                          f"{tuple(table.shape)}, {len_before.numel()}, {cu.numel()}")
+                          f"{tuple(shape)}, {len_before.numel()}, {cu.numel()}")
+    return shape[1]
 
 
 def rope_append_4bit(qkv: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int, attention_scaling: float, q_out: torch.Tensor,
@@ -1290,22 +1296,23 @@ def rope_append_4bit(qkv: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
     if (k_pool is None) != (v_pool is None):
         raise KernelError("the pools come as both of keys and values, or neither")
     write = k_pool is not None
-    cols = (heads + (2 * kv_heads if write else 0)) * head_dim
-    if qkv.dim() != 3 or tuple(qkv.shape[1:]) != (n_tokens, cols):
-        raise KernelError(f"qkv is {tuple(qkv.shape)}, expected [splits, {n_tokens}, {cols}]")
+    cols, shape = (heads + (2 * kv_heads if write else 0)) * head_dim, qkv.shape
+    if len(shape) != 3 or shape[1] != n_tokens or shape[2] != cols:
+        raise KernelError(f"qkv is {tuple(shape)}, expected [splits, {n_tokens}, {cols}]")
     if q_out.numel() != n_tokens * heads * head_dim:
         raise KernelError("q_out does not fit the tokens and heads")
     if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.numel() < rotary_dim // 2:
         raise KernelError(f"the rotary part must be even, at most {head_dim} numbers, and have half as many frequencies; got {rotary_dim} and {inv_freq.numel()}")
-    _need_aligned(q_out, "q_out")
+    if q_out.data_ptr() % 16:
+        raise KernelError("q_out must start on a 16-byte boundary")
     if write:
-        _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+        width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
     else:
-        _check_step(table, cu, len_before, sequences, status)
+        width, blocks = _check_step(table, cu, len_before, sequences, status), 0
     fn = _fn("cache_4bit", "tt_rope_append_4bit", "pilpiifppppiippiiiiiipp")
-    _check(fn(_ptr(qkv), qkv.shape[0], qkv.stride(0), _ptr(inv_freq), rotary_dim, 1 if interleaved else 0, attention_scaling, _ptr(q_out), _ptr(k_pool),
-              _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0] if write else 0, _ptr(cu), _ptr(len_before), sequences, n_tokens, heads,
-              kv_heads, head_dim, 1 if write else 0, _ptr(status), _stream()), "rope_append_4bit")
+    _check(fn(_ptr(qkv), shape[0], qkv.stride(0), _ptr(inv_freq), rotary_dim, 1 if interleaved else 0, attention_scaling, _ptr(q_out), _ptr(k_pool),
+              _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, n_tokens, heads, kv_heads, head_dim, 1 if write else 0,
+              _ptr(status), _stream()), "rope_append_4bit")
 
 
 def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
@@ -1318,17 +1325,18 @@ def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
     _need(keys, torch.bfloat16, "expanded keys")
     _need(values, torch.bfloat16, "expanded values")
     _need(table_tmp, torch.int32, "temporary table")
-    if keys.dim() != 4 or keys.shape[2] != BLOCK_TOKENS or keys.shape[3] not in CACHE_4BIT_DIMS:
-        raise KernelError(f"expanded keys must be [places, kv_heads, {BLOCK_TOKENS}, head size], got {tuple(keys.shape)}")
-    places, kv_heads, _, head_dim = keys.shape
-    if tuple(values.shape) != (places, kv_heads, head_dim, BLOCK_TOKENS) or tuple(table_tmp.shape) != tuple(table.shape) or places < sequences or places % sequences:
+    shape = keys.shape
+    if len(shape) != 4 or shape[2] != BLOCK_TOKENS or shape[3] not in CACHE_4BIT_DIMS:
+        raise KernelError(f"expanded keys must be [places, kv_heads, {BLOCK_TOKENS}, head size], got {tuple(shape)}")
+    places, kv_heads, _, head_dim = shape
+    if values.shape != (places, kv_heads, head_dim, BLOCK_TOKENS) or table_tmp.shape != table.shape or places < sequences or places % sequences:
         raise KernelError("expand_4bit: values, temporary table or number of places do not fit")
-    _need_aligned(keys, "expanded keys")
-    _need_aligned(values, "expanded values")
-    _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    if keys.data_ptr() % 16 or values.data_ptr() % 16:
+        raise KernelError("expanded keys and values must start on a 16-byte boundary")
+    width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
     fn = _fn("cache_4bit", "tt_expand_4bit", "pppiippiiiiippppp")
-    _check(fn(_ptr(k_pool), _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0], _ptr(cu), _ptr(len_before), sequences, kv_heads, head_dim,
-              window, places // sequences, _ptr(keys), _ptr(values), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
+    _check(fn(_ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, kv_heads, head_dim, window, places // sequences,
+              _ptr(keys), _ptr(values), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
 
 
 def attention_4bit_part_rows(device: torch.device | int | None = None) -> int:
@@ -1361,9 +1369,10 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         raise KernelError("one_token_each needs exactly one token per sequence")
     if not 0 <= splits <= 8:
         raise KernelError(f"keys are cut into 1 to 8 slices, or into even runs (0), not {splits}")
-    _need_aligned(q, "queries")
+    if q.data_ptr() % 16 or out.data_ptr() % 4:
+        raise KernelError("queries must start on a 16-byte boundary, the output on one of 4 bytes")
     _check_sinks(sinks, heads)
-    _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
     rows = 0
     if splits == 0:
         rows = attention_4bit_part_rows(q.device)
@@ -1375,7 +1384,7 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
             raise KernelError(f"attention_4bit: even runs need {4 * sm_count(q.device)} int32 tickets")
     wide = not one_token_each and n_tokens > sequences                 # several tokens of a sequence share a pass over its keys
     fn = _fn("attention_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppplppp")
-    _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), table.shape[1], k_pool.shape[0], _ptr(cu), _ptr(len_before), sequences, n_tokens,
+    _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, n_tokens,
               heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, 1 if wide else 0, _ptr(out), _ptr(part_acc), _ptr(part_ml),
               _ptr(tickets), rows, _ptr(status), _ptr(sinks), _stream()), "attention_4bit")
 
