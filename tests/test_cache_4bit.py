@@ -113,6 +113,38 @@ def test_reading_back_refuses(change, match):
         api.expand_4bit(**args)
 
 
+HALF = dict(keys=torch.zeros(4, 2, 64, 64, dtype=torch.float16), values=torch.zeros(4, 2, 64, 64, dtype=torch.float16), scales=torch.zeros(2, 4, 2),
+            marks=torch.zeros(4, 2, 64, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(keys=torch.zeros(4, 2, 64, 64, dtype=torch.bfloat16)), "float16"), (dict(scales=torch.zeros(2, 3, 2)), "scales"), (dict(scales=None), "bfloat16"),
+    (dict(marks=None), "marks"), (dict(marks=torch.zeros(4, 2, 32, dtype=torch.uint8)), "marks"), (dict(scales=torch.zeros(2, 4, 2, dtype=torch.float64)), "float32"),
+    (dict(keys=torch.zeros(4, 2, 64, 64, dtype=torch.bfloat16), values=torch.zeros(4, 2, 64, 64, dtype=torch.bfloat16), scales=None), "marks"),
+])
+def test_reading_back_float16_refuses(change, match):
+    args = dict(k_pool=torch.zeros(3, 2, 2560, dtype=torch.uint8), v_pool=torch.zeros(3, 2, 2560, dtype=torch.uint8), window=0,
+                table_tmp=torch.zeros(1, 3, dtype=torch.int32), **HALF, **step())
+    args.update(change)
+    with pytest.raises(api.KernelError, match=match):
+        api.expand_4bit(**args)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=torch.zeros(2, 256)), "does not take"), (dict(out=torch.zeros(2, 256)), "bfloat16"), (dict(out=torch.zeros(1, 256, dtype=torch.bfloat16)), "fit"),
+    (dict(n_tokens=3), "fit"), (dict(head_dim=80), "head"), (dict(heads=34, kv_heads=2), "does not take"), (dict(sinks=torch.zeros(3)), "sinks"),
+    (dict(scale=0.0), "positive"), (dict(scale=float("nan")), "positive"), (dict(scales=torch.zeros(4, 2)), "fit"), (dict(marks=torch.zeros(4, 2, 64)), "uint8"),
+    (dict(values=torch.zeros(3, 2, 64, 64, dtype=torch.float16)), "fit"), (dict(len_before=torch.zeros(1)), "int32"),
+    (dict(q=torch.zeros(520, dtype=torch.bfloat16)[4:516].view(2, 256)), "16-byte"), (dict(table=torch.zeros(2, 2, 2, dtype=torch.int32)), "row"),
+])
+def test_attention_over_float16_blocks_refuses(change, match):
+    args = dict(q=torch.zeros(2, 256, dtype=torch.bfloat16), n_tokens=2, heads=4, kv_heads=2, head_dim=64, scale=0.125, window=0,
+                out=torch.zeros(2, 256, dtype=torch.bfloat16), **HALF, **step())
+    args.update(change)
+    with pytest.raises(api.KernelError, match=match):
+        api.attention_half(**args)
+
+
 def test_what_a_4bit_call_would_do_on_the_cpu_is_an_error():
     with pytest.raises(api.KernelError):
         api.rope_append_4bit(**append_args())

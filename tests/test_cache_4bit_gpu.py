@@ -3,7 +3,8 @@
 Tolerances, derived from the kernels' roundings (a rounding is off by at most eps / 2 of its value: bf16 2^-8, fp16 2^-11, float32 2^-24).  Attention over 4 bits:
 the output 2^-8 of itself; the weights 2^-11 each, so 2^-11 of the sum of p (s n + |m|) (the second term's 16 bits are less); scores are float32 sums of at
 most 4 x (32 + 4) terms, so within 2^-24 * 160 of the terms' magnitudes, of which the exponentials and their sum take twice that and 2^-20 of their own.
-Through bfloat16 copies: keys 2^-8, which moves a score by 2^-8 of its terms' magnitudes and the output by twice that of its own; weights and values 2^-8 each."""
+Through copies of the blocks in 16 bits, to bfloat16's precision: keys 2^-8, which moves a score by 2^-8 of its terms' magnitudes and the output by twice that
+of its own; weights and values 2^-8 each (float16 blocks have bounds of their own, below)."""
 from __future__ import annotations
 
 import math
@@ -338,7 +339,7 @@ def test_sinks(splits):
 
 
 @pytest.mark.parametrize("q_scale,key_scale,value_scale", [(0.0, 1.0, 1.0), (1e-20, 1.0, 1.0), (30.0, 1.0, 1.0), (1e-3, 1e3, 1.0), (1e10, 1e-10, 1.0), (1.0, 1.0, 1e-15),
-                                                           (1.0, 1.0, 1e15), (1.0, 1.0, 1e-6), (1.0, 0.0, 0.0)])
+                                                           (1.0, 1.0, 1e15), (1.0, 1.0, 1e-6), (1.0, 0.0, 0.0), (1e4, 1e3, 1.0), (1e6, 1e6, 1.0)])
 @pytest.mark.parametrize("splits", [1, 0])
 def test_numbers_of_any_size(q_scale, key_scale, value_scale, splits):
     step = Step([400, 70], [1, 1], 2, 128, key_scale=key_scale, value_scale=value_scale)
@@ -502,6 +503,172 @@ def test_prompts_through_expanded_blocks(dim, kv, heads, before, new, options):
     out = torch.full_like(q, 7.0)
     mixer.attend(ctx, q, cache, step.table, out)
     close_to(out, step, q, heads, window=reach, expanded=True)
+
+
+def expanded(step, window=0, fill=7.0):
+    """The step's blocks as float16 numbers with scales and marks, and the table that names them."""
+    from thintensor_b200.kernels import api
+
+    places = len(step.new) * step.table.shape[1]
+    keys = torch.full((places, step.kv, 64, step.dim), fill, dtype=torch.float16, device=DEV)
+    values, named = torch.full((places, step.kv, step.dim, 64), fill, dtype=torch.float16, device=DEV), torch.full_like(step.table, 5)
+    scales, marks = torch.full((2, places, step.kv), 1.0, device=DEV), torch.zeros((places, step.kv, 64), dtype=torch.uint8, device=DEV)
+    api.expand_4bit(step.k_pool, step.v_pool, window=window, keys=keys, values=values, table_tmp=named, scales=scales, marks=marks, **step.common())
+    return keys, values, scales, marks, named
+
+
+def run_half(step, q, heads, window=0, sinks=None, out=None, n=None, fill=7.0):
+    from thintensor_b200.kernels import api
+
+    keys, values, scales, marks, named = expanded(step, window, fill)
+    out = torch.full_like(q, 7.0) if out is None else out
+    api.attention_half(q, keys, values, scales, marks, n_tokens=n or q.shape[0], heads=heads, kv_heads=step.kv, head_dim=step.dim, scale=step.dim ** -0.5, window=window,
+                       out=out, sinks=sinks, **(step.common() | dict(table=named)))
+    return out
+
+
+def close_to_half(got, step, q, heads, window=0, sinks=None):
+    """Output 2^-8; keys 2^-11, which moves a score by that much of its terms' magnitudes and the output by twice that of its own, with the float32 sums'
+    2^-16 beside it; weights, values and their sum 2^-11 each; a weight, kept
+    2^7 times as large, under float16's 2^-14 by 2^-25, which beside a value scaled by 2^8k less (at least 2^7 in size) is 2^-24 of the largest value."""
+    want, weight, reach = plain.attend(step.cache, q, step.before, step.new, heads, step.dim ** -0.5, window, sinks)
+    moved = (2.0 ** -11 + 2.0 ** -16) * reach[..., None]
+    largest = max(float((s.double() * 15).nan_to_num(0.0).abs().max() + m.double().nan_to_num(0.0).abs().max()) for _, s, m in [step.cache.v_parts])
+    allowed = 2.0 ** -8 * want.abs() + (torch.expm1(2 * moved) + 3 * 2.0 ** -11) * weight + max(step.totals) * 2.0 ** -24 * largest
+    off = (got.double().cpu().view_as(want) - want).abs()
+    assert bool((off <= allowed + 1e-30).all()), float((off / (allowed + 1e-30)).max())
+    assert int(step.status.item()) == 0
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("before,new,window", [([0, 130, 64], [1, 70, 1], 0), ([200, 64, 0], [1, 9, 3], 70), ([129, 300], [60, 1], -64)])
+@pytest.mark.parametrize("key_scale,value_scale", [(1.0, 1.0), (1e30, 1e-30), (0.0, 3e4)])
+def test_reading_back_float16_and_scales(dim, before, new, window, key_scale, value_scale):
+    step = Step(before, new, 3, dim, seed=7, key_scale=key_scale, value_scale=value_scale)
+    step.cache.poison("v", 0, step.totals[0] - 1, 1, 0)
+    step.k_pool, step.v_pool = step.cache.pools()
+    keys, values, scales, marks, named = expanded(step, window)
+    assert bool((scales[0] > 0).all()) and bool((torch.frexp(scales).mantissa.abs() == 0.5).all())
+    for b, total in enumerate(step.totals):
+        for w in range(plain.first_key(before[b], window) // 64, (total - 1) // 64 + 1):
+            place, block, upto = int(named[b, w]), int(step.cache.table[b, w]), min(64, total - 64 * w)
+            for h in range(3):
+                for i, (name, got) in enumerate((("k", keys[place, h]), ("v", values[place, h].T))):
+                    n, s, m = (t[block, h] for t in getattr(step.cache, name + "_parts"))
+                    want = plain.numbers(n, s, m)
+                    bad = torch.isnan(want)
+                    want[bad] = 0
+                    want[upto:] = 0
+                    scale = float(scales[i, place, h])
+                    off = (got.double().cpu() * abs(scale) - want).abs()
+                    # 11 bits, after a float32 multiply-add; under 2^-14 half of float16's last place
+                    assert bool((off <= (2.0 ** -11 + 2.0 ** -23) * want.abs() + 2.0 ** -25 * abs(scale)).all())
+                    if name == "v":
+                        mark = torch.stack([bad[:, 32 * g] for g in range(dim // 32)], 1)
+                        mark[upto:] = False
+                        assert (scale < 0) == bool(mark.any())
+                        if scale < 0:
+                            assert torch.equal(marks[place, h].cpu().long(), (mark.long() << torch.arange(dim // 32)).sum(1))
+    assert int(step.status.item()) == 0
+
+
+@pytest.mark.parametrize("dim,kv,heads", [(32, 2, 2), (64, 2, 8), (64, 3, 15), (96, 2, 6), (96, 1, 16), (128, 2, 8), (128, 1, 12), (128, 2, 14), (32, 1, 16)])
+@pytest.mark.parametrize("before,new", [([0], [1]), ([62, 0, 64, 5], [3, 130, 1, 0]), ([200, 0, 700], [17, 0, 33]), ([63], [300])])
+@pytest.mark.parametrize("window", [0, 1, 70, -64])
+def test_attention_over_float16_blocks(dim, kv, heads, before, new, window):
+    step = Step(before, new, kv, dim, seed=dim + heads)
+    for b, have in enumerate(before):
+        step.table[b, :plain.first_key(have, window) // 64] = -1
+    q = queries(step, heads)
+    more = torch.cat((q, q[:1]))                                       # a row behind the last sequence
+    got = run_half(step, more, heads, window=window)
+    close_to_half(got[:step.n], step, q, heads, window=window)
+    assert bool((got[step.n:] == 7.0).all())
+    # what stands in places that no block fills is never part of an output
+    assert torch.equal(run_half(step, q, heads, window=window, fill=math.nan), got[:step.n])
+
+
+@pytest.mark.parametrize("dim", [64, 96])
+@pytest.mark.parametrize("q_scale,key_scale,value_scale", [(0.0, 1.0, 1.0), (1e-20, 1.0, 1.0), (30.0, 1.0, 1.0), (1e-3, 1e3, 1.0), (1e10, 1e-10, 1.0), (1.0, 1.0, 1e-15),
+                                                           (1.0, 1.0, 1e15), (1.0, 1.0, 1e-6), (1.0, 0.0, 0.0), (1e30, 1e-30, 1e5), (1e-30, 1e30, 1e30), (1e-35, 1e-3, 1e-30), (1e4, 1e3, 1.0),
+                                                           (1e6, 1e6, 1.0)])
+def test_float16_blocks_of_any_size(dim, q_scale, key_scale, value_scale):
+    step = Step([300, 70], [40, 3], 2, dim, key_scale=key_scale, value_scale=value_scale)
+    q = queries(step, 8, scale=q_scale)
+    close_to_half(run_half(step, q, 8), step, q, 8)
+
+
+def test_float16_blocks_whose_scales_differ():
+    """Keys and values that grow by 2^3 from block to block, and rows of queries by 2^5 from token to token."""
+    for names, ways in (("k", (1, -1)), ("v", (1, -1)), ("kv", (1,))):
+        for way in ways:
+            step = Step([500], [20], 1, 64)
+            for name in names:
+                n, s, m = getattr(step.cache, name + "_parts")
+                for w in range(9):
+                    block, factor = int(step.cache.table[0, w]), 2.0 ** (way * (3 * w - 18))
+                    s[block], m[block] = s[block] * factor, m[block] * factor
+                setattr(step.cache, name + "_host", torch.stack([plain.write_block(n[i, 0], s[i, 0], m[i, 0], name == "v")[None] for i in range(n.shape[0])]))
+            step.k_pool, step.v_pool = step.cache.pools()
+            q = queries(step, 4) * (2.0 ** (5.0 * torch.arange(20, device=DEV) - 80))[:, None].bfloat16()
+            close_to_half(run_half(step, q, 4), step, q, 4)
+
+
+def test_float16_blocks_with_sinks():
+    step = Step([300, 2, 64], [10, 30, 1], 2, 64)
+    sinks = torch.tensor([0.0, 5.0, -3.0, 40.0, -40.0, 1.0, 2.0, 0.5], device=DEV)
+    q = queries(step, 8)
+    close_to_half(run_half(step, q, 8, sinks=sinks), step, q, 8, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_what_is_not_a_number_in_a_prompt(dim):
+    step = Step([300, 20, 0], [30, 100, 5], 2, dim)
+    q = queries(step, 8)
+    window = 100
+    clean = run_half(step, q, 8, window=window).clone()
+    step.cache.poison("v", 0, 300 - window, 0, 0)                      # before the first row's window, in its first block
+    step.cache.poison("k", 0, 300 - window, 1, 0)
+    step.cache.poison("v", 1, 60, 1, dim // 32 - 1)                    # seen by its own token and the 99 after it
+    step.cache.poison("k", 1, 90, 0, 0)
+    step.k_pool, step.v_pool = step.cache.pools()
+    q[132] = q[132].clone()
+    q[132, 3 * dim + 5] = math.inf                                     # the third sequence's third token, its fourth head
+    got = run_half(step, q, 8, window=window).view(-1, 8, dim)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    position = torch.arange(20, 120, device=DEV)
+    bad[30:130, 4:, dim - 32:] = ((position >= 60) & (position < 160))[:, None, None]
+    bad[30:130, :4] |= (position >= 90)[:, None, None]
+    bad[132, 3] = True
+    assert torch.equal(torch.isnan(got), bad) and torch.equal(got[~bad], clean.view_as(got)[~bad])
+    assert int(step.status.item()) == 0
+
+
+def test_float16_blocks_outside_the_places_are_flagged():
+    from thintensor_b200.kernels import api
+
+    step = Step([100], [50], 2, 64)
+    step.table[0, 1] = 1 << 20
+    run_half(step, queries(step, 8), 8)
+    assert int(step.status.item()) == api.STATUS_BAD_BLOCK
+
+
+def test_prompts_captured_and_replayed_for_other_lengths():
+    step = Step([170, 90], [40, 60], 2, 96)
+    mixer, ctx, cache = layer(step, 8, False)
+    q = queries(step, 8)
+    out = torch.full_like(q, 7.0)
+    mixer.attend(ctx, q, cache, step.table, out)
+    close_to_half(out, step, q, 8)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mixer.attend(ctx, q, cache, step.table, out)
+    for before in ([1, 70], [0, 0], [170, 90]):
+        step.before, step.totals = before, [before[0] + 40, before[1] + 60]
+        step.len_before.copy_(ints(before))
+        out.fill_(7.0)
+        graph.replay()
+        close_to_half(out, step, q, 8)
 
 
 def test_which_way_a_step_goes():

@@ -221,10 +221,10 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            m_new[e] = fmaxf(st.m_run[nq][e], mx * st.scale[nq][e]);   // the scale is positive
+            m_new[e] = fmaxf(st.m_run[nq][e], __fmul_ru(mx, st.scale[nq][e]));   // the scale is positive; rounded up, so that no weight leaves float16's reach
             corr[nq][e] = m_new[e] == -INFINITY ? 1.0f : fast_exp2((st.m_run[nq][e] - m_new[e]) + (e_old - e_now));
             grew = grew || corr[nq][e] != 1.0f;
-            base[e] = m_new[e] == -INFINITY ? 0.0f : -(m_new[e] + e_now);
+            base[e] = m_new[e] == -INFINITY ? 0.0f : -__fadd_ru(m_new[e], e_now);
         }
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -676,7 +676,7 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             for (int dt = 0; dt < 2 * G; ++dt)
                 if (!DUP || ((dt >> 1) & 1) == (c >> 1)) { dst[16 * dt] = st.o[dt][nq][e]; dst[16 * dt + 8] = st.o[dt][nq][2 + e]; }
             if (r == 0 && (!DUP || c < 2)) {
-                sh_m[warp * COLS + col] = st.m_run[nq][e] + (float)(st.e_run - 14);
+                sh_m[warp * COLS + col] = __fadd_ru(st.m_run[nq][e], (float)(st.e_run - 14));
                 sh_l[warp * COLS + col] = st.l_run[nq][e];
             }
         }

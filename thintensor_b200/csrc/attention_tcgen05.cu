@@ -25,8 +25,15 @@
 // At the end every thread divides its row of O by the row sum and stores it.
 // Every wait is bounded as in gemm_tcgen05.cu.
 //
+// The HALF instances read what expand_4bit_kernel made of a 4-bit cache: keys and values in float16 with a power of two a block and head, since a
+// number of such a cache is a sum that bfloat16 would round once more (the outputs' error against 64 bits: 0.0039 with bfloat16 blocks and weights,
+// 0.0017 with these, which is the rounding of the outputs).  The softmax threads bring their rows of queries to float16 in place, with a power of two
+// a row, before the first product; the weights are float16 too.
+//
 // The reference has no counterpart: it feeds prompts token by token through its
 // single-token attention (thinruntime/cli.py:2802-2807, thinruntime/triton_kernels.py:14-109).
+#include <cuda_fp16.h>
+#include "cache_4bit.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -109,11 +116,17 @@ struct Args {
     const float* gate;
     int gate_splits, gate_row, gate_per_head;
     long long gate_split_stride;
+    // the HALF instances only: float32 powers of two that a block's numbers are to be multiplied by, [keys or values][pool_blocks][kv_heads], and the
+    // numbers of a head (HD, or fewer: the rest of a row is read as zeros, or not used).  A values' scale below zero: groups of 32 numbers of some tokens
+    // are NaN and read as zeros, block_marks [pool_blocks][kv_heads][64] has a bit for each
+    const float* block_scales;
+    const uint8_t* block_marks;
+    int dim;
     float* maps;            // the MAPS instance's output: [2][tokens][heads][128]
     int n_tokens;
 };
 
-template <int HD, bool SHAPED, bool MAPS = false>
+template <int HD, bool SHAPED, bool MAPS = false, bool HALF = false>
 __global__ void __launch_bounds__(Layout<HD, MAPS>::THREADS, HD == 64 ? 2 : 1)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const Args args) {
@@ -127,6 +140,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __shared__ uint32_t tmem_base_shared;
     __shared__ int tile_info[2];                                  // sequence, tile within the sequence
     __shared__ float pair_max[2][2][ROWS];
+    __shared__ uint64_t q_ready;                                  // HALF: the queries have been converted
 
     tt_pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -161,6 +175,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&q_full), 1);
+        if (HALF) mbar_init(smem_u32(&q_ready), 4 * L::SPLIT);
         for (int s = 0; s < KV_STAGES; ++s) { mbar_init(smem_u32(&kv_full[s]), 1); mbar_init(smem_u32(&kv_empty[s]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&p_ready[i]), 4 * L::SPLIT); mbar_init(smem_u32(&pv_done[i]), 1); }
         fence_barrier_init();
@@ -209,7 +224,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const uint32_t bar = smem_u32(&kv_full[s]);
                 mbar_expect_tx(bar, L::STAGE_BYTES);
                 uint8_t* stage = kv_smem + (size_t)s * L::STAGE_BYTES;
-                const int k_row = (block * args.kv_heads + kh) * KEYS, v_row = (block * args.kv_heads + kh) * VD;
+                const int k_row = (block * args.kv_heads + kh) * KEYS, v_row = (block * args.kv_heads + kh) * (HALF ? args.dim : VD);
 #pragma unroll
                 for (int c = 0; c < L::CHUNKS; ++c) tma_load_2d(smem_u32(stage + c * KEYS * 128), &map_k, map_col + c * 64, k_row, bar);
                 tma_load_2d(smem_u32(stage + L::K_BYTES), &map_v, 0, v_row, bar);
@@ -221,8 +236,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         if (lane == 0) {
-            constexpr uint32_t idesc_s = instr_desc(ROWS, KEYS), idesc_o = instr_desc(ROWS, VD);
-            bool ok = mbar_wait(smem_u32(&q_full), 0);
+            constexpr uint32_t TYPES = HALF ? ~((1u << 7) | (1u << 10)) : ~0u;        // both operands float16, or both bfloat16
+            constexpr uint32_t idesc_s = instr_desc(ROWS, KEYS) & TYPES, idesc_o = instr_desc(ROWS, VD) & TYPES;
+            bool ok = mbar_wait(smem_u32(HALF ? &q_ready : &q_full), 0);
             if (!ok) atomicOr(args.status, TT_STATUS_WAIT_EXPIRED);
             auto issue_s = [&](int i) {                           // S_i = Q K_i^T into S accumulator i & 1
                 const int s = i % KV_STAGES;
@@ -274,7 +290,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         float m_used = -INFINITY, l = 0.0f;                       // the scale in use (log2 units) and this thread's part of the sum
         bool ok = true;
         // shaped scores are brought to log2 units key by key, so the scale that follows is one
-        const float scale_log2 = SHAPED ? 1.0f : args.scale_log2;
+        float scale_log2 = SHAPED ? 1.0f : args.scale_log2;
         float slope_log2 = 0.0f, inv_cap = 0.0f;
         if (SHAPED) {
             if (args.slopes) slope_log2 = __ldg(args.slopes + kh * args.group + (r - local * args.group)) * 1.4426950408889634f;
@@ -282,7 +298,71 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         auto pair_barrier = [&]() { if (SPLIT == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
         auto expired = [&]() { if (lane == 0) atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; };
+        const int* table_row = args.table + (size_t)b * args.table_width + block0;
+        float row_scale = 1.0f, value_scale = 1.0f, next_key = 1.0f, next_value = 1.0f;
+        int this_block = 0, next_block = 0;
+        unsigned not_numbers = 0;                                 // groups of 32 numbers of the row's output
+        // a block outside the pool is read as block 0 (and flagged) by the thread that loads it
+        auto scales_at = [&](int i) {
+            const int block = i < n_blocks ? __ldg(table_row + i) : 0;
+            return (block >= 0 && block < args.pool_blocks ? block : 0) * args.kv_heads + kh;
+        };
+        if constexpr (HALF) {
+            const float* value_scales = args.block_scales + (size_t)args.pool_blocks * args.kv_heads;
+            this_block = scales_at(0);
+            next_key = __ldg(args.block_scales + this_block);
+            next_value = __ldg(value_scales + this_block);
+            next_block = scales_at(1);
+            // O is in units of the largest scale of the values that the tile sees
+            value_scale = 0.0f;
+            for (int i = lane; i < n_blocks; i += 32) value_scale = fmaxf(value_scale, fabsf(__ldg(value_scales + scales_at(i))));
+            value_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(value_scale)));
+            // 64 numbers of the row's queries a thread, 16 bytes a time, each thread from another bank
+            if (!mbar_wait(smem_u32(&q_full), 0)) expired();
+            uint8_t* row = q_smem + half * ROWS * 128 + r * 128;
+            uint4 x[8];
+            uint32_t most = 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                x[u] = *reinterpret_cast<const uint4*>(row + ((u + lane) & 7) * 16);
+                most = __vmaxu2(most, __vmaxu2(__vmaxu2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu), __vmaxu2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu)));
+            }
+            float largest = __uint_as_float(max(most & 0xffffu, most >> 16) << 16);
+            if (SPLIT == 2) {
+                pair_max[1][half][r] = largest;
+                pair_barrier();
+                largest = __uint_as_float(max(__float_as_uint(largest), __float_as_uint(pair_max[1][half ^ 1][r])));     // (a NaN stays)
+            }
+            if (!(largest < INFINITY)) not_numbers = ~0u;
+            const int e = cache4::half_exponent(largest);
+            row_scale = cache4::power_of_two(e) * args.scale_log2;
+            const float down = cache4::power_of_two(-e);
+            auto two = [&](uint32_t w) {
+                const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+                return *reinterpret_cast<const uint32_t*>(&h);
+            };
+#pragma unroll
+            for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(row + ((u + lane) & 7) * 16) = make_uint4(two(x[u].x), two(x[u].y), two(x[u].z), two(x[u].w));
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(smem_u32(&q_ready));
+        }
         for (int i = 0; i < n_blocks; ++i) {
+            float value_part = 1.0f;
+            if constexpr (HALF) {
+                // neither infinite nor zero, so that a masked score stays what it is (scores of that size are infinite or zero themselves)
+                scale_log2 = fminf(fmaxf(row_scale * next_key, 1e-36f), 1e36f);
+                value_part = __fdividef(fabsf(next_value), value_scale);  // powers of two, at most one
+                if (next_value < 0.0f) {
+                    const uint8_t* marks = args.block_marks + (size_t)this_block * KEYS;
+                    const int key0 = (block0 + i) * KEYS;
+                    for (int j = max(0, first - key0); j < KEYS && key0 + j <= pos; ++j) not_numbers |= marks[j];
+                }
+                this_block = next_block;
+                next_key = __ldg(args.block_scales + next_block);
+                next_value = __ldg(args.block_scales + (size_t)args.pool_blocks * args.kv_heads + next_block);
+                next_block = scales_at(i + 2);
+            }
             if (ok && !mbar_wait(smem_u32(&s_full[i & 1]), (uint32_t)((i >> 1) & 1))) expired();
             fence_after_sync();
             float s[HALF_KEYS];
@@ -368,10 +448,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 pair_barrier();
                 mx = fmaxf(mx, pair_max[i & 1][half ^ 1][r]);
             }
-            mx *= scale_log2;
-            const bool grow = mx > m_used + RESCALE_THRESHOLD || (m_used == -INFINITY && mx != -INFINITY);
+            // HALF: the largest weight in use is 2^7 when its scale is new and never more than 2^15, float16's reach, however large the scores are (so
+            // what is taken off a score is rounded up); weights under 2^-21 of the largest are the first that float16 holds with fewer bits
+            mx = HALF ? __fmul_ru(mx, scale_log2) : mx * scale_log2;
+            const bool grow = mx > (HALF ? __fadd_rd(m_used, 7.0f + RESCALE_THRESHOLD) : m_used + RESCALE_THRESHOLD) || (m_used == -INFINITY && mx != -INFINITY);
             if (__any_sync(0xffffffffu, grow)) {
-                const float m_new = grow ? mx : m_used;
+                const float m_new = grow ? (HALF ? __fadd_ru(mx, -7.0f) : mx) : m_used;
                 const float corr = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
                 if (i > 0) {
                     if (ok && !mbar_wait(smem_u32(&pv_done[(i - 1) & 1]), (uint32_t)(((i - 1) >> 1) & 1))) expired();
@@ -404,8 +486,21 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if ((j >> 1) & 1) sum_b = add2(sum_b, p); else sum_a = add2(sum_a, p);
                 float p0, p1;
                 unpack2(p, p0, p1);
-                const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-                packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                if constexpr (HALF) {
+                    const __half2 h = __floats2half2_rn(p0, p1);
+                    packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+                    packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            if (HALF && value_part != 1.0f) {                             // rare: scales go in steps of 2^8
+                const __half2 part = __float2half2_rn(value_part);
+#pragma unroll
+                for (int j = 0; j < HALF_KEYS / 2; ++j) {
+                    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&packed[j]), part);
+                    packed[j] = *reinterpret_cast<const uint32_t*>(&h);
+                }
             }
             {
                 float a0, a1;
@@ -437,7 +532,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (ok) {
             fence_after_sync();
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * value_scale;
             const int token = seq_begin + tok0 + local, head = kh * args.group + (r - local * args.group);
             if constexpr (MAPS) {
                 float* dst = args.maps + (((size_t)(blockIdx.x & 1) * args.n_tokens + token) * args.heads + head) * VD;
@@ -462,6 +557,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int c = 0; c < O_COLS; c += 32) {
                 float o[32];
                 tmem_load32(lane_base + L::O_COL + half * O_COLS + c, o);
+                if (HALF && (not_numbers >> ((half * O_COLS + c) / 32) & 1))
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(0x7fc00000u);
                 if (gated) {
                     if (args.gate_per_head) {
 #pragma unroll
@@ -519,10 +617,11 @@ differential_combine_kernel(const float* __restrict__ maps, long long rows, floa
     *reinterpret_cast<uint2*>(out + row * 128 + c) = *reinterpret_cast<uint2*>(v);
 }
 
-template <int HD, bool SHAPED, bool MAPS = false>
+template <int HD, bool SHAPED, bool MAPS = false, bool HALF = false>
 int launch(const void* q, const void* k_pool, const void* v_pool, const Args& args, int n_tokens, cudaStream_t stream) {
     using L = Layout<HD, MAPS>;
-    constexpr int ROW = MAPS ? 2 * HD : HD;                      // numbers of a row of q or k
+    const int ROW = HALF ? args.dim : MAPS ? 2 * HD : HD;        // numbers of a row of q or k
+    const int value_dim = HALF ? args.dim : L::VD;
     CUtensorMap map_q, map_k, map_v;
     {   // q [token][head][dim]: a box of 64 dims x group heads x tokens_per_tile tokens = up to 128 rows of 128 bytes
         const cuuint64_t dims[3] = {(cuuint64_t)ROW, (cuuint64_t)args.heads, (cuuint64_t)n_tokens};
@@ -537,12 +636,12 @@ int launch(const void* q, const void* k_pool, const void* v_pool, const Args& ar
         if (!tc::make_map(&map_k, k_pool, 2, dims, strides, box)) return -1;
     }
     {   // values [block * kv_head * dim][64 tokens]
-        const cuuint64_t dims[2] = {(cuuint64_t)KEYS, (cuuint64_t)args.pool_blocks * args.kv_heads * L::VD};
+        const cuuint64_t dims[2] = {(cuuint64_t)KEYS, (cuuint64_t)args.pool_blocks * args.kv_heads * value_dim};
         const cuuint64_t strides[1] = {(cuuint64_t)KEYS * 2};
         const cuuint32_t box[2] = {KEYS, (cuuint32_t)L::VD};
         if (!tc::make_map(&map_v, v_pool, 2, dims, strides, box)) return -1;
     }
-    auto kernel = attention_tcgen05_kernel<HD, SHAPED, MAPS>;
+    auto kernel = attention_tcgen05_kernel<HD, SHAPED, MAPS, HALF>;
     const cudaError_t err = tt_allow_shared(kernel, L::SMEM);
     if (err != cudaSuccess) return (int)err;
     tt_launch_pdl(kernel, dim3(args.kv_heads * (MAPS ? 2 : 1), args.cta_tiles), dim3(L::THREADS), (size_t)L::SMEM, stream, map_q, map_k, map_v, args);
@@ -585,6 +684,28 @@ extern "C" int tt_attention_tcgen05(const void* q, const void* k_pool, const voi
     }
     if (head_dim == 64) return launch<64, false>(q, k_pool, v_pool, args, n_tokens, stream);
     return launch<128, false>(q, k_pool, v_pool, args, n_tokens, stream);
+}
+
+// The same over the float16 blocks that tt_expand_4bit makes of a 4-bit cache (32, 64, 96 or 128 numbers a head): keys [places][kv_heads][64][head_dim],
+// values [places][kv_heads][head_dim][64], scales float32 [2][places][kv_heads], marks [places][kv_heads][64], and the table of places that it fills.
+extern "C" int tt_attention_half(const void* q, const void* keys, const void* values, const float* scales, const uint8_t* marks, const int* table, int table_width, int places,
+                                 const int* cu, const int* len_before, int sequences, int n_tokens, int heads, int kv_heads, int head_dim, float scale,
+                                 const float* sinks, int window, void* out, unsigned* status, cudaStream_t stream) {
+    if (n_tokens <= 0) return 0;
+    if (!cache4::takes(heads, kv_heads, head_dim) || !scales || !marks ||
+        (((uintptr_t)q | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out) & 15) || (long long)places * kv_heads > (2147483647LL - 128) / head_dim)
+        return (int)cudaErrorInvalidValue;
+    Args args = {};
+    args.out_dim = args.dim = head_dim; args.block_scales = scales; args.block_marks = marks;
+    args.table = table; args.table_width = table_width; args.pool_blocks = places; args.cu = cu; args.len_before = len_before;
+    args.sequences = sequences; args.heads = heads; args.kv_heads = kv_heads; args.group = heads / kv_heads;
+    args.tokens_per_tile = ROWS / args.group;
+    args.cta_tiles = (n_tokens + args.tokens_per_tile - 1) / args.tokens_per_tile + sequences;
+    if (args.cta_tiles > 65535) return (int)cudaErrorInvalidValue;
+    args.scale_log2 = scale * 1.4426950408889634f; args.window = window; args.out = (__nv_bfloat16*)out; args.status = status; args.sinks = sinks;
+    args.scale = scale;
+    if (head_dim <= 64) return launch<64, false, false, true>(q, keys, values, args, n_tokens, stream);
+    return launch<128, false, false, true>(q, keys, values, args, n_tokens, stream);
 }
 
 // Differential attention of packed prompts, bfloat16, two maps of 64 numbers over values of 128: q [tokens][heads][2 x 64], key rows of 2 x 64 numbers.

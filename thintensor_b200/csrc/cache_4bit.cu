@@ -1,5 +1,6 @@
 // A block cache whose keys and values are held in 4 bits (see cache_4bit.cuh): writing it (with the rotation) and reading it back.  Head sizes 32,
 // 64, 96 and 128, bfloat16 queries.
+#include <cuda_fp16.h>
 #include "cache_4bit.cuh"
 
 namespace {
@@ -276,12 +277,27 @@ rope_append_4bit_kernel(const float* __restrict__ qkv, int splits, size_t split_
 // those: block w of sequence b goes to place b * span + w - (its first block that is seen), and table_tmp names the places (-1: not
 // seen, or outside the pool).  Tokens behind the sequence's end become zeros.  Bound by the 16 bits a number that it writes.
 // grid = (2 * span, kv_heads, sequences): keys and values are CTAs of their own.
-template <int D>
+// HALF: float16 numbers instead, each times a power of two of its block and head, whose inverse goes to scales [keys or values][places][kv_heads]
+// (a bfloat16 number would be m + s n rounded once more, to 8 bits; these have 11).  A group of values that is not a number becomes zeros, so that a
+// product with a weight of zero is zero: the block's scale is then negative, and marks [places][kv_heads][64] names such groups of every token.
+template <bool HALF>
+__device__ __forceinline__ uint32_t two_numbers(float a, float b) {
+    if constexpr (HALF) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+template <int D, bool HALF>
 __global__ void __launch_bounds__(256)
 expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, const int* __restrict__ table, int table_width,
                    int pool_blocks, const int* __restrict__ cu, const int* __restrict__ len_before, int kv_heads, int window, int span,
-                   __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values, int* __restrict__ table_tmp, unsigned* status) {
+                   uint16_t* __restrict__ keys, uint16_t* __restrict__ values, float* __restrict__ scales, uint8_t* __restrict__ marks, int* __restrict__ table_tmp, unsigned* status) {
     constexpr int G = D / 32;
+    __shared__ float most[8];
     tt_pdl_wait();
     tt_pdl_launch_dependents();
     const int b = blockIdx.z, kh = blockIdx.y, place = blockIdx.x >> 1;
@@ -304,28 +320,63 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
     }
     const int left = length - w * TT_BLOCK_TOKENS;                     // tokens of this block
     const size_t from = ((size_t)block * kv_heads + kh) * block_bytes(D), to = ((size_t)(b * span + place) * kv_heads + kh) * TT_BLOCK_TOKENS * D;
-    if (!(blockIdx.x & 1)) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pool + from);
-        const uint32_t* pairs = words + code_bytes(D) / 4;
+    const bool of_keys = !(blockIdx.x & 1);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>((of_keys ? k_pool : v_pool) + from);
+    const uint32_t* pairs = words + code_bytes(D) / 4;                 // of keys
+    const __nv_bfloat16* tops = reinterpret_cast<const __nv_bfloat16*>(words + code_bytes(D) / 4);            // of values
+    const __nv_bfloat16* least = tops + TT_BLOCK_TOKENS * G;
+    float down = 1.0f;
+    if constexpr (HALF) {
+        // the largest number of the block: a thread a group of a token
+        float mine = 0.0f;
+        bool bad = false;
+        const int token = threadIdx.x / G, g = threadIdx.x % G;
+        if (threadIdx.x < TT_BLOCK_TOKENS * G && token < left) {
+            float s, m;
+            if (of_keys) {
+                const uint32_t pair = __ldg(pairs + threadIdx.x);
+                s = __uint_as_float(pair << 16);
+                m = __uint_as_float(pair & 0xffff0000u);
+            } else {
+                s = __bfloat162float(tops[threadIdx.x]);
+                m = __bfloat162float(least[g * TT_BLOCK_TOKENS + token]);
+            }
+            bad = s != s;
+            if (!bad) mine = fmaxf(fabsf(m), fabsf(fmaf(15.0f, s, m)));
+        }
+        const uint32_t warp_most = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
+        if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = __uint_as_float(warp_most);
+        const bool any_bad = __syncthreads_or(bad) && !of_keys;
+        float largest = most[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) largest = fmaxf(largest, most[k]);
+        const int e = cache4::half_exponent(largest);
+        down = cache4::power_of_two(-e);
+        const size_t slot = ((size_t)b * span + place) * kv_heads + kh;
+        if (threadIdx.x == 0) scales[(of_keys ? 0 : (size_t)gridDim.z * span * kv_heads) + slot] = any_bad ? -cache4::power_of_two(e) : cache4::power_of_two(e);
+        if (any_bad && threadIdx.x < TT_BLOCK_TOKENS) {
+            unsigned mask = 0;
+            for (int k = 0; k < G; ++k) mask |= (unsigned)(threadIdx.x < left && tops[threadIdx.x * G + k] != tops[threadIdx.x * G + k]) << k;
+            marks[slot * TT_BLOCK_TOKENS + threadIdx.x] = (uint8_t)mask;
+        }
+    }
+    if (of_keys) {
 #pragma unroll
         for (int k = 0; k < G; ++k) {
             const int i = k * 256 + threadIdx.x;
             const int c = i & 3, g = (i >> 2) % G, token = (i >> 2) / G;       // eight neighbouring numbers
             const uint32_t word = __ldg(words + (token * 4 + c) * G + g), pair = __ldg(pairs + token * G + g);
-            const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
+            const float s = __uint_as_float(pair << 16) * down, m = __uint_as_float(pair & 0xffff0000u) * down;
             uint32_t out[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 two = __floats2bfloat162_rn(fmaf(s, (float)((word >> (4 * e)) & 15u), m), fmaf(s, (float)((word >> (4 * e + 16)) & 15u), m));
-                out[e] = token < left ? *reinterpret_cast<const uint32_t*>(&two) : 0u;
+                const uint32_t two = two_numbers<HALF>(fmaf(s, (float)((word >> (4 * e)) & 15u), m), fmaf(s, (float)((word >> (4 * e + 16)) & 15u), m));
+                out[e] = token < left ? two : 0u;
             }
             *reinterpret_cast<uint4*>(keys + to + (size_t)token * D + 32 * g + 8 * c) = make_uint4(out[0], out[1], out[2], out[3]);
         }
         return;
     }
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(v_pool + from);
-    const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(words + code_bytes(D) / 4);
-    const __nv_bfloat16* least = scales + TT_BLOCK_TOKENS * G;
     const int c = threadIdx.x & 3, a = (threadIdx.x >> 2) & 3, r = (threadIdx.x >> 4) & 7, jj = threadIdx.x >> 7, token = 16 * a + 4 * c;
 #pragma unroll
     for (int g = 0; g < G; ++g) {                                      // four tokens of two numbers
@@ -334,17 +385,14 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
         const float m[4] = {__uint_as_float(low.x << 16), __uint_as_float(low.x & 0xffff0000u), __uint_as_float(low.y << 16), __uint_as_float(low.y & 0xffff0000u)};
         float s[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] = __bfloat162float(scales[(token + k) * G + g]);
+        for (int k = 0; k < 4; ++k) s[k] = __bfloat162float(tops[(token + k) * G + g]) * down;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float x[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                x[k] = token + k < left ? fmaf(s[k], (float)((word >> (4 * (2 * (k >> 1) + e) + 16 * (k & 1))) & 15u), m[k]) : 0.0f;
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-            uint2 v;
-            v.x = *reinterpret_cast<const uint32_t*>(&lo);
-            v.y = *reinterpret_cast<const uint32_t*>(&hi);
+                x[k] = token + k < left && (!HALF || s[k] == s[k]) ? fmaf(s[k], (float)((word >> (4 * (2 * (k >> 1) + e) + 16 * (k & 1))) & 15u), m[k] * down) : 0.0f;
+            const uint2 v = make_uint2(two_numbers<HALF>(x[0], x[1]), two_numbers<HALF>(x[2], x[3]));
             *reinterpret_cast<uint2*>(values + to + (size_t)(32 * g + 16 * jj + 8 * e + r) * TT_BLOCK_TOKENS + token) = v;
         }
     }
@@ -381,16 +429,18 @@ extern "C" int tt_rope_append_4bit(const float* qkv, int splits, long long split
     TT_LAUNCH_CHECK();
 }
 
+// scales, marks: null for bfloat16 keys and values, else those of float16 ones.
 extern "C" int tt_expand_4bit(const void* k_pool, const void* v_pool, const int* table, int table_width, int pool_blocks, const int* cu,
                               const int* len_before, int sequences, int kv_heads, int head_dim, int window, int span, void* keys, void* values,
-                              int* table_tmp, unsigned* status, cudaStream_t stream) {
+                              float* scales, uint8_t* marks, int* table_tmp, unsigned* status, cudaStream_t stream) {
     if (sequences <= 0) return 0;
-    if (!cache4::takes(kv_heads, kv_heads, head_dim) || span < 1 || sequences > 65535 || (((uintptr_t)keys | (uintptr_t)values) & 15) != 0) return (int)cudaErrorInvalidValue;
+    if (!cache4::takes(kv_heads, kv_heads, head_dim) || span < 1 || sequences > 65535 || (scales != nullptr) != (marks != nullptr) || (((uintptr_t)keys | (uintptr_t)values) & 15) != 0) return (int)cudaErrorInvalidValue;
     if (span > (1 << 29)) return (int)cudaErrorInvalidValue;
     const dim3 grid(2 * span, kv_heads, sequences);
-#define TT_LAUNCH(D)                                                                                                                             \
-    tt_launch_pdl(expand_4bit_kernel<D>, grid, dim3(256), 0, stream, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, \
-                  cu, len_before, kv_heads, window, span, (__nv_bfloat16*)keys, (__nv_bfloat16*)values, table_tmp, status)
+#define TT_LAUNCH_T(D, H)                                                                                                                           \
+    tt_launch_pdl(expand_4bit_kernel<D, H>, grid, dim3(256), 0, stream, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, \
+                  cu, len_before, kv_heads, window, span, (uint16_t*)keys, (uint16_t*)values, scales, marks, table_tmp, status)
+#define TT_LAUNCH(D) (scales ? TT_LAUNCH_T(D, true) : TT_LAUNCH_T(D, false))
     switch (head_dim) {
         case 32: TT_LAUNCH(32); break;
         case 64: TT_LAUNCH(64); break;
@@ -398,5 +448,6 @@ extern "C" int tt_expand_4bit(const void* k_pool, const void* v_pool, const int*
         default: TT_LAUNCH(128); break;
     }
 #undef TT_LAUNCH
+#undef TT_LAUNCH_T
     TT_LAUNCH_CHECK();
 }

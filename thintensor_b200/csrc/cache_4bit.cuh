@@ -27,6 +27,14 @@ namespace cache4 {
 constexpr int block_bytes(int d) { return 40 * d; }                 // of one head's keys, or values
 constexpr int code_bytes(int d) { return 32 * d; }                  // the codes among them
 
+// Numbers of at most this size are held in float16 times 2^-e: the largest then lies in 2^7 .. 2^15, so that what is 2^-21 of it still has float16's 11
+// bits.  e is a multiple of 8, so that most blocks of a cache have the same one; a scale and its inverse are normal float32 numbers.
+__device__ __forceinline__ int half_exponent(float largest) {
+    const int exponent = (int)(__float_as_uint(largest) >> 23) - 127;
+    return max(-112, ((exponent - 7) >> 3) * 8);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 inline bool takes(int heads, int kv_heads, int head_dim) {
     return kv_heads > 0 && kv_heads <= 65535 && heads % kv_heads == 0 && heads / kv_heads >= 1 && heads / kv_heads <= 16 &&
            (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128);

@@ -1316,14 +1316,19 @@ def rope_append_4bit(qkv: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
 
 
 def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
-                window: int, keys: torch.Tensor, values: torch.Tensor, table_tmp: torch.Tensor, status: torch.Tensor) -> None:
+                window: int, keys: torch.Tensor, values: torch.Tensor, table_tmp: torch.Tensor, status: torch.Tensor,
+                scales: torch.Tensor | None = None, marks: torch.Tensor | None = None) -> None:
     """The blocks of a cache in 4 bits that a step's queries see, as bfloat16 blocks: ``keys`` ``[places, kv_heads, 64, head_dim]`` and ``values``
     ``[places, kv_heads, head_dim, 64]`` with ``places`` a multiple of ``sequences``: a sequence's blocks, from the first that it sees (``window`` as in
     :func:`attention`), lie side by side in its ``places / sequences`` places (a step that sees more flags a bad shape), tokens behind its end
     are zero, and places that it does not fill stay as they are.  ``table_tmp`` (int32, like ``table``) names the place of every block, -1 for those not
-    seen: with it, ``keys`` and ``values`` are what a plain cache's pools and table would be."""
-    _need(keys, torch.bfloat16, "expanded keys")
-    _need(values, torch.bfloat16, "expanded values")
+    seen: with it, ``keys`` and ``values`` are what a plain cache's pools and table would be.  With ``scales`` (float32 ``[2, places, kv_heads]``) and
+    ``marks`` (uint8 ``[places, kv_heads, 64]``) ``keys`` and ``values`` are float16 instead, to be multiplied by the power of two of their place and head
+    (``scales[0]`` the keys', ``scales[1]`` the values'): three bits more of every number, for :func:`attention_half`.  Groups of values that are NaN
+    are zeros there, the place's scale is negative, and the token's mark has the group's bit."""
+    dtype = torch.bfloat16 if scales is None else torch.float16
+    _need(keys, dtype, "expanded keys")
+    _need(values, dtype, "expanded values")
     _need(table_tmp, torch.int32, "temporary table")
     shape = keys.shape
     if len(shape) != 4 or shape[2] != BLOCK_TOKENS or shape[3] not in CACHE_4BIT_DIMS:
@@ -1331,12 +1336,51 @@ def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
     places, kv_heads, _, head_dim = shape
     if values.shape != (places, kv_heads, head_dim, BLOCK_TOKENS) or table_tmp.shape != table.shape or places < sequences or places % sequences:
         raise KernelError("expand_4bit: values, temporary table or number of places do not fit")
+    if (scales is None) != (marks is None):
+        raise KernelError("expand_4bit: scales and marks go together")
+    if scales is not None:
+        _need(scales, torch.float32, "scales of the expanded blocks")
+        _need(marks, torch.uint8, "marks of the expanded blocks")
+        if scales.shape != (2, places, kv_heads) or marks.shape != (places, kv_heads, BLOCK_TOKENS):
+            raise KernelError(f"the scales of {places} places of {kv_heads} heads are [2, {places}, {kv_heads}] and their marks [{places}, {kv_heads}, {BLOCK_TOKENS}], "
+                              f"got {tuple(scales.shape)} and {tuple(marks.shape)}")
     if keys.data_ptr() % 16 or values.data_ptr() % 16:
         raise KernelError("expanded keys and values must start on a 16-byte boundary")
     width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
-    fn = _fn("cache_4bit", "tt_expand_4bit", "pppiippiiiiippppp")
+    fn = _fn("cache_4bit", "tt_expand_4bit", "pppiippiiiiippppppp")
     _check(fn(_ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, kv_heads, head_dim, window, places // sequences,
-              _ptr(keys), _ptr(values), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
+              _ptr(keys), _ptr(values), _ptr(scales), _ptr(marks), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
+
+
+def attention_half(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, marks: torch.Tensor, table: torch.Tensor,
+                   cu: torch.Tensor, len_before: torch.Tensor, sequences: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int, scale: float, window: int,
+                   out: torch.Tensor, status: torch.Tensor, sinks: torch.Tensor | None = None) -> None:
+    """Causal attention of packed bfloat16 prompts over the float16 blocks, their scales, marks and the table that :func:`expand_4bit` made of a
+    cache in 4 bits: :func:`attention_tcgen05` with float16 products, whose weights, keys and values are rounded to 11 bits instead of 8.  ``window``,
+    ``sinks``: see :func:`attention`."""
+    if not cache_4bit_supports(q.dtype, heads, kv_heads, head_dim):
+        raise KernelError(f"attention over float16 blocks does not take {q.dtype}, {heads}/{kv_heads} heads of size {head_dim}")
+    _check_sinks(sinks, heads)
+    _need(q, torch.bfloat16, "queries")
+    _need(out, torch.bfloat16, "output")
+    _need(keys, torch.float16, "expanded keys")
+    _need(values, torch.float16, "expanded values")
+    _need(scales, torch.float32, "scales of the expanded blocks")
+    _need(marks, torch.uint8, "marks of the expanded blocks")
+    places = keys.shape[0]
+    if keys.shape != (places, kv_heads, BLOCK_TOKENS, head_dim) or values.shape != (places, kv_heads, head_dim, BLOCK_TOKENS) or \
+            scales.shape != (2, places, kv_heads) or marks.shape != (places, kv_heads, BLOCK_TOKENS):
+        raise KernelError(f"attention_half: keys, values, scales and marks do not fit {kv_heads} heads of {head_dim}")
+    if q.numel() != n_tokens * heads * head_dim or out.numel() != q.numel():
+        raise KernelError("attention_half: queries or output do not fit the heads")
+    if not scale > 0.0:
+        raise KernelError(f"the scale of the scores must be positive, got {scale}")
+    _check_step(table, cu, len_before, sequences, status)
+    if any(t.data_ptr() % 16 for t in (q, keys, values, out)):
+        raise KernelError("queries, expanded keys and values and the output must start on a 16-byte boundary")
+    fn = _fn("attention_tcgen05", "tt_attention_half", "ppppppiippiiiiifpippp")
+    _check(fn(_ptr(q), _ptr(keys), _ptr(values), _ptr(scales), _ptr(marks), _ptr(table), table.shape[1], places, _ptr(cu), _ptr(len_before), sequences, n_tokens,
+              heads, kv_heads, head_dim, scale, _ptr(sinks), window, _ptr(out), _ptr(status), _stream()), "attention_half")
 
 
 def attention_4bit_part_rows(device: torch.device | int | None = None) -> int:

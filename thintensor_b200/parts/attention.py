@@ -352,11 +352,9 @@ class CausalAttention(Mixer):
         return min(width, (ctx.n_tokens - ctx.sequences + 1 + bound - 1 + 62) // 64 + 1)
 
     def expands_4bit(self, ctx, width: int) -> bool:
-        """Whether a step's prompts go through bfloat16 copies of the blocks that they see: the 4-bit kernel reads a sequence's cache
-        once for every few tokens, the copies are read by kernels that take a hundred at a time (with sinks: the tcgen05 kernel alone)."""
+        """Whether a step's prompts go through float16 copies of the blocks that they see: the 4-bit kernel reads a sequence's cache
+        once for every few tokens, the copies are read by the tcgen05 kernel, which takes many at a time."""
         if ctx.decode or ctx.n_tokens < self.EXPAND_4BIT_FROM * ctx.sequences:
-            return False
-        if self.sinks is not None and not api.attention_tcgen05_supports(torch.bfloat16, self.heads, self.kv_heads, self.head_dim):
             return False
         return ctx.sequences * self.span_4bit(ctx, width) * 64 * self.kv_heads * self.head_dim * 4 <= self.EXPAND_4BIT_BYTES
 
@@ -364,16 +362,15 @@ class CausalAttention(Mixer):
         width = table.shape[1]
         if self.expands_4bit(ctx, width):
             places = ctx.sequences * self.span_4bit(ctx, width)
-            keys = ctx.scratch("attention.keys", (places, self.kv_heads, 64, self.head_dim))
-            values = ctx.scratch("attention.values", (places, self.kv_heads, self.head_dim, 64))
             named = ctx.scratch("attention.table", tuple(table.shape), torch.int32)
-            api.expand_4bit(cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, self.reach, keys, values, named, ctx.status)
-            if api.attention_tcgen05_supports(q.dtype, self.heads, self.kv_heads, self.head_dim):
-                api.attention_tcgen05(q, keys, values, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
-                                      self.head_dim, self.scale, self.reach, mixed, ctx.status, sinks=self.sinks)
-            else:
-                api.attention_mma(q, keys, values, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
-                                  self.head_dim, self.scale, self.reach, 1, mixed, None, None, ctx.status)
+            keys = ctx.scratch("attention.keys", (places, self.kv_heads, 64, self.head_dim), torch.float16)
+            values = ctx.scratch("attention.values", (places, self.kv_heads, self.head_dim, 64), torch.float16)
+            scales = ctx.scratch("attention.scales", (2, places, self.kv_heads), torch.float32)
+            marks = ctx.scratch("attention.marks", (places, self.kv_heads, 64), torch.uint8)
+            api.expand_4bit(cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, self.reach, keys, values, named, ctx.status,
+                            scales=scales, marks=marks)
+            api.attention_half(q, keys, values, scales, marks, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
+                               self.head_dim, self.scale, self.reach, mixed, ctx.status, sinks=self.sinks)
             return
         group, sms = self.heads // self.kv_heads, api.sm_count(ctx.status.device)
         wide = group > 8 or ctx.n_tokens > ctx.sequences               # tiles of up to 16 rows, of which an SM holds half as many
