@@ -42,7 +42,6 @@ using namespace tc;
 
 constexpr int ROWS = 128;            // query rows of a CTA
 constexpr int KEYS = TT_BLOCK_TOKENS;
-constexpr int KV_STAGES = 3;
 constexpr float RESCALE_THRESHOLD = 8.0f;     // in log2 units
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -78,7 +77,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // MAPS (head size 64 only): two attention maps a head over the same values, of twice a map's size (differential attention): a CTA makes one of them,
 // float32, and differential_combine_kernel the heads' outputs.  P lies over the score accumulator that it was made from, which its thread has read and
 // which is not written again before the products of P are done, so that O's 128 columns leave room for a second CTA on the SM.
-template <int HD, bool MAPS = false> struct Layout {
+// HALF at head size 128 (APART): P lies over the scores too, and there are two stages instead of three, whose keys and values are waited for and given back
+// each by itself (keys as soon as their scores are made): a second CTA fits an SM, and one's products run beside the other's exponentials.  2,048 tokens
+// behind 1,000, 32/8 heads: 84 us, twice the products' floor; one CTA with three stages 108 us, two with stages of keys and values together 93 us; two tiles of rows
+// in one CTA over four stages of the same keys and values 85 us, so it is neither the loads nor the shared memory: exponentials take 40 % of their unit's time,
+// issue slots are 46 % used, and the last tiles leave SMs with one CTA or none (the SMs are at work 84 % of the time).
+template <int HD, bool MAPS = false, bool HALF = false> struct Layout {
     // Threads per query row in the softmax.  Head size 128 leaves room for one CTA per SM only, and
     // four softmax warps cannot hide their own latencies: two threads per row (8 warps) are 10 %
     // faster there.  Head size 64 runs two CTAs per SM and is bound elsewhere: one thread per row.
@@ -89,11 +93,16 @@ template <int HD, bool MAPS = false> struct Layout {
     static constexpr int VD = MAPS ? 2 * HD : HD;               // numbers of a value
     static constexpr int K_BYTES = KEYS * HD * 2;
     static constexpr int STAGE_BYTES = K_BYTES + KEYS * VD * 2;
+    static constexpr bool APART = HALF && HD == 128;
+    static constexpr int KV_STAGES = APART ? 2 : 3;
     static constexpr int SMEM = Q_BYTES + KV_STAGES * STAGE_BYTES + 1024;
     static constexpr int O_COL = 128;                           // S: 2 x 64 columns, then O: HD, then P: 2 x 32 (bfloat16 pairs)
-    static constexpr int P_COL = MAPS ? 0 : O_COL + HD, P_STEP = MAPS ? 64 : 32;
+    static constexpr bool P_OVER_S = MAPS || APART;
+    static constexpr int P_COL = P_OVER_S ? 0 : O_COL + HD, P_STEP = P_OVER_S ? 64 : 32;
     static_assert(!MAPS || HD == 64, "two maps a head: of 64 numbers each");
-    static constexpr int TMEM_COLS = HD == 64 ? 256 : 512;
+    static constexpr int TMEM_COLS = HD == 64 || APART ? 256 : 512;
+    static constexpr int TAKEN = APART ? 16 : 32;                 // columns of O that are rescaled at a time (APART leaves 96 registers a thread)
+    static constexpr int CTAS = HD == 64 || APART ? 2 : 1;        // on an SM
 };
 
 struct Args {
@@ -127,11 +136,12 @@ struct Args {
 };
 
 template <int HD, bool SHAPED, bool MAPS = false, bool HALF = false>
-__global__ void __launch_bounds__(Layout<HD, MAPS>::THREADS, HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(Layout<HD, MAPS, HALF>::THREADS, Layout<HD, MAPS, HALF>::CTAS)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const Args args) {
-    using L = Layout<HD, MAPS>;
-    constexpr int VD = L::VD;
+    using L = Layout<HD, MAPS, HALF>;
+    constexpr int VD = L::VD, KV_STAGES = L::KV_STAGES;
+    constexpr bool APART = L::APART;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_smem = smem;
@@ -141,6 +151,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __shared__ int tile_info[2];                                  // sequence, tile within the sequence
     __shared__ float pair_max[2][2][ROWS];
     __shared__ uint64_t q_ready;                                  // HALF: the queries have been converted
+    __shared__ uint64_t v_full[KV_STAGES], v_empty[KV_STAGES];    // APART: the values'; kv_full and kv_empty are the keys'
 
     tt_pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -176,6 +187,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&q_full), 1);
         if (HALF) mbar_init(smem_u32(&q_ready), 4 * L::SPLIT);
+        if (APART) for (int s = 0; s < KV_STAGES; ++s) { mbar_init(smem_u32(&v_full[s]), 1); mbar_init(smem_u32(&v_empty[s]), 1); }
         for (int s = 0; s < KV_STAGES; ++s) { mbar_init(smem_u32(&kv_full[s]), 1); mbar_init(smem_u32(&kv_empty[s]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&p_ready[i]), 4 * L::SPLIT); mbar_init(smem_u32(&pv_done[i]), 1); }
         fence_barrier_init();
@@ -221,17 +233,27 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 int block = table_row[walk_back ? block1 - i : block0 + i];
                 if (block < 0 || block >= args.pool_blocks) { atomicOr(args.status, TT_STATUS_BAD_BLOCK); block = 0; }
-                const uint32_t bar = smem_u32(&kv_full[s]);
-                mbar_expect_tx(bar, L::STAGE_BYTES);
+                uint32_t bar = smem_u32(&kv_full[s]);
+                mbar_expect_tx(bar, APART ? L::K_BYTES : L::STAGE_BYTES);
                 uint8_t* stage = kv_smem + (size_t)s * L::STAGE_BYTES;
                 const int k_row = (block * args.kv_heads + kh) * KEYS, v_row = (block * args.kv_heads + kh) * (HALF ? args.dim : VD);
 #pragma unroll
                 for (int c = 0; c < L::CHUNKS; ++c) tma_load_2d(smem_u32(stage + c * KEYS * 128), &map_k, map_col + c * 64, k_row, bar);
+                if (APART) {
+                    if (i >= KV_STAGES && !mbar_wait(smem_u32(&v_empty[s]), (uint32_t)(((i / KV_STAGES) & 1) ^ 1))) {
+                        atomicOr(args.status, TT_STATUS_WAIT_EXPIRED);
+                        mbar_wait(bar, (uint32_t)((i / KV_STAGES) & 1));         // its keys are on their way
+                        break;
+                    }
+                    bar = smem_u32(&v_full[s]);
+                    mbar_expect_tx(bar, L::STAGE_BYTES - L::K_BYTES);
+                }
                 tma_load_2d(smem_u32(stage + L::K_BYTES), &map_v, 0, v_row, bar);
                 ++issued;
             }
             for (int i = max(0, issued - KV_STAGES); i < issued; ++i)       // drain before shared memory is given up
-                if (!mbar_wait(smem_u32(&kv_full[i % KV_STAGES]), (uint32_t)((i / KV_STAGES) & 1))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); break; }
+                if (!mbar_wait(smem_u32(&kv_full[i % KV_STAGES]), (uint32_t)((i / KV_STAGES) & 1)) ||
+                    (APART && !mbar_wait(smem_u32(&v_full[i % KV_STAGES]), (uint32_t)((i / KV_STAGES) & 1)))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); break; }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
@@ -251,23 +273,25 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     umma_bf16(tmem_base + (i & 1) * 64, smem_desc(q_addr + off_q), smem_desc(k_addr + off_k), idesc_s, kk > 0 ? 1u : 0u);
                 }
                 umma_commit(smem_u32(&s_full[i & 1]));
+                if (APART) umma_commit(smem_u32(&kv_empty[s]));
             };
             if (ok) issue_s(0);
             if (ok && n_blocks > 1) issue_s(1);
             for (int i = 0; i < n_blocks && ok; ++i) {
                 // O += P_i V_i once the softmax warps have written P_i
                 if (!mbar_wait(smem_u32(&p_ready[i & 1]), (uint32_t)((i >> 1) & 1))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; break; }
-                fence_after_sync();
                 const int s = i % KV_STAGES;
+                if (APART && !mbar_wait(smem_u32(&v_full[s]), (uint32_t)((i / KV_STAGES) & 1))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; break; }
+                fence_after_sync();
                 const uint32_t p_tmem = tmem_base + L::P_COL + (i & 1) * L::P_STEP;
                 const uint32_t v_addr = smem_u32(kv_smem + (size_t)s * L::STAGE_BYTES + L::K_BYTES);
 #pragma unroll
                 for (int kk = 0; kk < KEYS / 16; ++kk)
                     umma_bf16_a_in_tmem(tmem_base + L::O_COL, p_tmem + kk * 8, smem_desc(v_addr + kk * 32), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
-                umma_commit(smem_u32(&kv_empty[s]));              // K_i and V_i are free once these products are done
+                umma_commit(smem_u32(APART ? &v_empty[s] : &kv_empty[s]));   // K_i and V_i are free once these products are done
                 umma_commit(smem_u32(&pv_done[i & 1]));
                 // P_i lies in the next but one block's score accumulator: the products that read it must be done
-                if (MAPS && i + 2 < n_blocks && !mbar_wait(smem_u32(&pv_done[i & 1]), (uint32_t)((i >> 1) & 1))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; break; }
+                if (L::P_OVER_S && i + 2 < n_blocks && !mbar_wait(smem_u32(&pv_done[i & 1]), (uint32_t)((i >> 1) & 1))) { atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; break; }
                 if (i + 2 < n_blocks) issue_s(i + 2);             // its S accumulator was read before P_i was announced
             }
         }
@@ -459,12 +483,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     if (ok && !mbar_wait(smem_u32(&pv_done[(i - 1) & 1]), (uint32_t)(((i - 1) >> 1) & 1))) expired();
                     fence_after_sync();
 #pragma unroll
-                    for (int c = 0; c < O_COLS; c += 32) {
-                        float o[32];
-                        tmem_load32(lane_base + L::O_COL + half * O_COLS + c, o);
+                    for (int c = 0; c < O_COLS; c += L::TAKEN) {
+                        const uint32_t at = lane_base + L::O_COL + half * O_COLS + c;
+                        float o[L::TAKEN];
+                        if constexpr (L::APART) tmem_load16(at, o); else tmem_load32(at, o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= corr;
-                        tmem_store32(lane_base + L::O_COL + half * O_COLS + c, o);
+                        for (int e = 0; e < L::TAKEN; ++e) o[e] *= corr;
+                        if constexpr (L::APART) tmem_store16(at, reinterpret_cast<const uint32_t*>(o)); else tmem_store32(at, o);
                     }
                 }
                 l *= corr;
@@ -510,7 +535,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // P_i goes to buffer i & 1, which the products of block i - 2 must have finished reading.  They have: the
             // issuing thread asked for them before it asked for S_i, its products complete in the order it issues them, and
             // this thread has seen S_i complete.  (A wait of its own on pv_done here cost 160 cycles of 1,500 a block.)
-            if (SPLIT == 2) tmem_store16(lane_base + L::P_COL + (i & 1) * 32 + half * 16, packed);
+            if (SPLIT == 2) tmem_store16(lane_base + L::P_COL + (i & 1) * L::P_STEP + half * 16, packed);
             else tmem_store32(lane_base + L::P_COL + (i & 1) * L::P_STEP, reinterpret_cast<const float*>(packed));
             fence_before_sync();
             __syncwarp();
@@ -619,7 +644,7 @@ differential_combine_kernel(const float* __restrict__ maps, long long rows, floa
 
 template <int HD, bool SHAPED, bool MAPS = false, bool HALF = false>
 int launch(const void* q, const void* k_pool, const void* v_pool, const Args& args, int n_tokens, cudaStream_t stream) {
-    using L = Layout<HD, MAPS>;
+    using L = Layout<HD, MAPS, HALF>;
     const int ROW = HALF ? args.dim : MAPS ? 2 * HD : HD;        // numbers of a row of q or k
     const int value_dim = HALF ? args.dim : L::VD;
     CUtensorMap map_q, map_k, map_v;
