@@ -241,3 +241,20 @@ def test_storage_of_a_4bit_group():
 ])
 def test_the_plain_choice(logits, u, settings, want):
     assert plain.choose(torch.tensor(logits), u, **settings) == want
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (32, 8), (16, 2), (32, 2)])
+def test_slices_of_a_step(heads, kv_heads):
+    """Slices are taken while their clusters are resident together and have 256 keys each; even runs for long caches alone."""
+    for sequences in (1, 2, 7, 40, 300):
+        for new in (1, 3, 24):
+            for longest in (1, 255, 511, 512, 3000, 8191, 8192, 40000):
+                splits = api.attention_4bit_splits(sequences, sequences * new, heads, kv_heads, longest, 148)
+                assert splits in (0, 1, 2, 4, 8)
+                if splits == 0:
+                    assert longest >= 8192 and sequences * kv_heads <= 4 * 148
+                else:
+                    assert splits == 1 or (longest >= 256 * splits and sequences * kv_heads * splits <= 4 * 148)
+    assert api.attention_4bit_splits(1, 1, heads, kv_heads, 2048, 148) == 8
+    assert api.attention_4bit_splits(1, 1, heads, kv_heads, 100, 148) == 1
+    assert api.attention_4bit_splits(2000, 2000, heads, kv_heads, 100000, 148) == 1

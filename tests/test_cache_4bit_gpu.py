@@ -495,14 +495,15 @@ def layer(step, heads, decode, **options):
 def test_prompts_through_expanded_blocks(dim, kv, heads, before, new, options):
     step = Step(before, new, kv, dim)
     mixer, ctx, cache = layer(step, heads, False, **options)
-    assert mixer.expands_4bit(ctx, step.table.shape[1])
     reach = mixer.reach
     for b, have in enumerate(before):
         step.table[b, :plain.first_key(have, reach) // 64] = -1
     q = queries(step, heads)
-    out = torch.full_like(q, 7.0)
-    mixer.attend(ctx, q, cache, step.table, out)
-    close_to(out, step, q, heads, window=reach, expanded=True)
+    for copies in (True, False):                                       # both ways that a prompt of this size could go
+        mixer.expands_4bit = lambda ctx, width: copies  # noqa: B023
+        out = torch.full_like(q, 7.0)
+        mixer.attend(ctx, q, cache, step.table, out)
+        close_to(out, step, q, heads, window=reach, expanded=copies)
 
 
 def expanded(step, window=0, fill=7.0):
@@ -653,9 +654,39 @@ def test_float16_blocks_outside_the_places_are_flagged():
     assert int(step.status.item()) == api.STATUS_BAD_BLOCK
 
 
+def test_a_table_too_narrow_for_the_lengths_is_flagged():
+    from thintensor_b200.kernels import api
+
+    step = Step([10], [300], 2, 64)
+    q = queries(step, 8)
+    keys, values, scales, marks, named = expanded(step)
+    padded = torch.full((4, 2), 1 << 20, dtype=torch.int32, device=DEV)      # what lies behind the row is never taken for a block
+    padded[0] = named[0, :2]
+    api.attention_half(q, keys, values, scales, marks, n_tokens=step.n, heads=8, kv_heads=2, head_dim=64, scale=0.125, window=0, out=torch.empty_like(q),
+                       **(step.common() | dict(table=padded[:1])))
+    assert int(step.status.item()) == api.STATUS_BAD_BLOCK
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    from thintensor_b200.kernels import api
+
+    step = Step([10], [20], 2, 64)
+    q, blocks = queries(step, 8), expanded(step)
+    logits = torch.randn(2, 100, device=DEV)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    calls = [lambda: append(step, torch.empty(1, 20, 12 * 64, device=DEV), 8, 0), lambda: run_attention(step, q, 8), lambda: expanded(step),
+             lambda: api.attention_half(q, *blocks[:4], n_tokens=20, heads=8, kv_heads=2, head_dim=64, scale=0.125, window=0, out=torch.empty_like(q),
+                                        **(step.common() | dict(table=blocks[4]))),
+             lambda: api.sample_filtered(logits, 1.0, 0, 1.0, 0.0, torch.empty(2, dtype=torch.int32, device=DEV), uniform=torch.zeros(2, device=DEV))]
+    for call in calls:
+        with pytest.raises(api.KernelError, match="the current device is cuda:1"):
+            call()
+
+
 def test_prompts_captured_and_replayed_for_other_lengths():
     step = Step([170, 90], [40, 60], 2, 96)
     mixer, ctx, cache = layer(step, 8, False)
+    mixer.expands_4bit = lambda ctx, width: True
     q = queries(step, 8)
     out = torch.full_like(q, 7.0)
     mixer.attend(ctx, q, cache, step.table, out)
@@ -674,13 +705,14 @@ def test_prompts_captured_and_replayed_for_other_lengths():
 def test_which_way_a_step_goes():
     step = Step([0], [100], 2, 64)
     mixer, ctx, cache = layer(step, 8, False)
+    ctx.n_tokens = 4096
     assert mixer.expands_4bit(ctx, 4) and mixer.span_4bit(ctx, 4) == 4
     assert not mixer.expands_4bit(ctx, 1 << 24)                        # copies that would not fit their scratch memory
     ctx.n_tokens = 15
     assert not mixer.expands_4bit(ctx, 4)
     windowed, ctx, _ = layer(step, 8, False, window=100)
     assert windowed.span_4bit(ctx, 1000) == (100 + 100 - 1 + 62) // 64 + 1
-    ctx.decode = True
+    ctx.n_tokens, ctx.decode = 4096, True
     assert not windowed.expands_4bit(ctx, 4)
 
 

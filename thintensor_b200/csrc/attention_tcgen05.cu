@@ -231,7 +231,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (i >= KV_STAGES && !mbar_wait(smem_u32(&kv_empty[s]), (uint32_t)(((i / KV_STAGES) & 1) ^ 1))) {
                     atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); break;
                 }
-                int block = table_row[walk_back ? block1 - i : block0 + i];
+                const int place = walk_back ? block1 - i : block0 + i;
+                int block = place < args.table_width ? table_row[place] : -1;
                 if (block < 0 || block >= args.pool_blocks) { atomicOr(args.status, TT_STATUS_BAD_BLOCK); block = 0; }
                 uint32_t bar = smem_u32(&kv_full[s]);
                 mbar_expect_tx(bar, APART ? L::K_BYTES : L::STAGE_BYTES);
@@ -322,13 +323,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         auto pair_barrier = [&]() { if (SPLIT == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
         auto expired = [&]() { if (lane == 0) atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; };
-        const int* table_row = args.table + (size_t)b * args.table_width + block0;
+        const int* table_row = args.table + (size_t)b * args.table_width;
         float row_scale = 1.0f, value_scale = 1.0f, next_key = 1.0f, next_value = 1.0f;
         int this_block = 0, next_block = 0;
         unsigned not_numbers = 0;                                 // groups of 32 numbers of the row's output
         // a block outside the pool is read as block 0 (and flagged) by the thread that loads it
         auto scales_at = [&](int i) {
-            const int block = i < n_blocks ? __ldg(table_row + i) : 0;
+            const int block = i < n_blocks && block0 + i < args.table_width ? __ldg(table_row + block0 + i) : 0;
             return (block >= 0 && block < args.pool_blocks ? block : 0) * args.kv_heads + kh;
         };
         if constexpr (HALF) {

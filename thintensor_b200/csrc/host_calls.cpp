@@ -188,6 +188,21 @@ static PyObject* host_tiled_operands(PyObject* module, PyObject* const* args, Py
     return PyBool_FromLong(tiled_rows(*x) && tiled_rows(*w) && x->size(1) % 8 == 0);
 }
 
+// the index of the device on which all CUDA tensors among the arguments lie; -1 without any, an error where they lie on several
+static PyObject* host_common_device(PyObject* module, PyObject* const* args, Py_ssize_t n) {
+    long common = -1;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (args[i] == Py_None) continue;
+        const at::Tensor* tensor = tensor_of(args[i]);
+        if (!tensor) return NULL;
+        if (!tensor->is_cuda()) continue;
+        const long index = tensor->get_device();
+        if (common >= 0 && index != common) return PyErr_Format(error_class, "tensors lie on cuda:%ld and on cuda:%ld", common, index);
+        common = index;
+    }
+    return PyLong_FromLong(common);
+}
+
 static PyObject* host_set_error(PyObject* module, PyObject* error) {
     Py_INCREF(error);
     Py_XSETREF(error_class, error);
@@ -199,6 +214,7 @@ static PyMethodDef methods[] = {
     {"need", (PyCFunction)(void (*)(void))guarded<host_need>, METH_FASTCALL, "Check a tensor's dtype and contiguity."},
     {"need_columns", (PyCFunction)(void (*)(void))guarded<host_need_columns>, METH_FASTCALL, "Check a tensor's dtype and that its columns lie side by side."},
     {"tiled_operands", (PyCFunction)(void (*)(void))guarded<host_tiled_operands>, METH_FASTCALL, "Whether two matrices can be the operands of a tiled bfloat16 product."},
+    {"common_device", (PyCFunction)(void (*)(void))guarded<host_common_device>, METH_FASTCALL, "The device of all CUDA tensors among the arguments; -1 without any."},
     {"set_error", host_set_error, METH_O, "The exception class for refused tensors."},
     {NULL, NULL, 0, NULL},
 };

@@ -166,11 +166,11 @@ _CTYPES = {"p": c_void_p, "i": c_int, "l": c_longlong, "u": c_ulonglong, "f": c_
 
 def _bind_host() -> None:
     """Take the native module's checks and calls; without a C++ compiler or Python's headers ctypes makes the same calls, slower."""
-    global _host, _ptr, _need, _need_columns
+    global _host, _ptr, _need, _need_columns, _common_device
     module = build.host_calls()
     if module is not None:
         module.set_error(KernelError)
-        _ptr, _need, _need_columns = module.pointer, module.need, module.need_columns
+        _ptr, _need, _need_columns, _common_device = module.pointer, module.need, module.need_columns, module.common_device
     _host = module or False
 
 
@@ -1253,6 +1253,20 @@ def cache_4bit_bytes(head_dim: int) -> int:
     return BLOCK_TOKENS * (head_dim // 2 + head_dim // 32 * 4)
 
 
+def _common_device(*tensors: torch.Tensor | None) -> int:
+    found = {t.get_device() for t in tensors if t is not None and t.is_cuda}
+    if len(found) > 1:
+        raise KernelError("tensors lie on " + " and on ".join(f"cuda:{i}" for i in sorted(found)))
+    return found.pop() if found else -1
+
+
+def _check_device(*tensors: torch.Tensor | None) -> None:
+    """The launch goes to the current device's stream, so everything has to lie there (what is on the CPU is refused when its address is taken)."""
+    device = _common_device(*tensors)
+    if device >= 0 and device != torch._C._cuda_getDevice():
+        raise KernelError(f"the tensors lie on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
 def _check_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor, len_before: torch.Tensor, sequences: int,
                 kv_heads: int, head_dim: int, status: torch.Tensor) -> tuple[int, int]:
     """Checks a step over a cache in 4 bits; returns the table's width and the pools' blocks."""
@@ -1309,6 +1323,7 @@ def rope_append_4bit(qkv: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
         width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
     else:
         width, blocks = _check_step(table, cu, len_before, sequences, status), 0
+    _check_device(qkv, inv_freq, q_out, k_pool, v_pool, table, cu, len_before, status)
     fn = _fn("cache_4bit", "tt_rope_append_4bit", "pilpiifppppiippiiiiiipp")
     _check(fn(_ptr(qkv), shape[0], qkv.stride(0), _ptr(inv_freq), rotary_dim, 1 if interleaved else 0, attention_scaling, _ptr(q_out), _ptr(k_pool),
               _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, n_tokens, heads, kv_heads, head_dim, 1 if write else 0,
@@ -1347,6 +1362,7 @@ def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
     if keys.data_ptr() % 16 or values.data_ptr() % 16:
         raise KernelError("expanded keys and values must start on a 16-byte boundary")
     width, blocks = _check_4bit(k_pool, v_pool, table, cu, len_before, sequences, kv_heads, head_dim, status)
+    _check_device(k_pool, v_pool, table, cu, len_before, keys, values, scales, marks, table_tmp, status)
     fn = _fn("cache_4bit", "tt_expand_4bit", "pppiippiiiiippppppp")
     _check(fn(_ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, kv_heads, head_dim, window, places // sequences,
               _ptr(keys), _ptr(values), _ptr(scales), _ptr(marks), _ptr(table_tmp), _ptr(status), _stream()), "expand_4bit")
@@ -1378,6 +1394,7 @@ def attention_half(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, sc
     _check_step(table, cu, len_before, sequences, status)
     if any(t.data_ptr() % 16 for t in (q, keys, values, out)):
         raise KernelError("queries, expanded keys and values and the output must start on a 16-byte boundary")
+    _check_device(q, keys, values, scales, marks, table, cu, len_before, sinks, out, status)
     fn = _fn("attention_tcgen05", "tt_attention_half", "ppppppiippiiiiifpippp")
     _check(fn(_ptr(q), _ptr(keys), _ptr(values), _ptr(scales), _ptr(marks), _ptr(table), table.shape[1], places, _ptr(cu), _ptr(len_before), sequences, n_tokens,
               heads, kv_heads, head_dim, scale, _ptr(sinks), window, _ptr(out), _ptr(status), _stream()), "attention_half")
@@ -1386,6 +1403,29 @@ def attention_half(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, sc
 def attention_4bit_part_rows(device: torch.device | int | None = None) -> int:
     """Rows of scratch memory that :func:`attention_4bit` wants for even runs: two for each query row of a tile and each CTA of the device."""
     return 64 * sm_count(device)
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_4bit_splits(sequences: int, n_tokens: int, heads: int, kv_heads: int, longest: int, sms: int) -> int:
+    """``splits`` for :func:`attention_4bit`, from a step's shape: ``longest`` is how many keys a token sees at most.  Slices in powers of two while all
+    clusters of them are resident at once, each of 256 keys at least: a cluster lies within 18 SMs, which hold 4 CTAs each, or 2 of the form for more than
+    eight query rows, and half as many of the form with eight warps that the kernel takes while there is an SM for each CTA.  Even runs for long caches that
+    would fill the GPU with less than its CTAs.  (440 shapes of 1 to 40 sequences, 1 to 24 tokens and 300 to 20,000 keys: 3.5 % above
+    the fastest of 0 to 8 in the mean, 1.7 times at most.)"""
+    group = heads // kv_heads
+    wide = group > 8 or n_tokens > sequences
+    tokens = 1 if n_tokens == sequences else (16 if wide else 8) // group          # of a tile
+    tiles = sequences * -(-n_tokens // (sequences * tokens)) * kv_heads
+    launched = tiles if n_tokens == sequences else (n_tokens // tokens + sequences) * kv_heads
+    if longest >= 8192 and longest * tiles >= 8 * 24576 and tiles <= (2 if wide else 4) * sms:
+        return 0
+    best = 1
+    for splits in (2, 4, 8):
+        single = launched * splits <= sms
+        held = (2 if wide else 4) // (2 if single else 1)
+        if longest // 256 >= splits and (launched if single else tiles) <= max(1, sms // 18) * (18 * held // splits):
+            best = splits
+    return best
 
 
 def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor, cu: torch.Tensor,
@@ -1427,6 +1467,7 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         if tickets is None or tickets.dtype != torch.int32 or tickets.numel() < 4 * sm_count(q.device):
             raise KernelError(f"attention_4bit: even runs need {4 * sm_count(q.device)} int32 tickets")
     wide = not one_token_each and n_tokens > sequences                 # several tokens of a sequence share a pass over its keys
+    _check_device(q, k_pool, v_pool, table, cu, len_before, out, part_acc, part_ml, tickets, sinks, status)
     fn = _fn("attention_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppplppp")
     _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, n_tokens,
               heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, 1 if wide else 0, _ptr(out), _ptr(part_acc), _ptr(part_ml),
@@ -2007,6 +2048,7 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k, top_p, min_p, out:
                 raise KernelError(f"{rows} rows need as many {name}, got {t.numel()}")
     if rows == 0:
         return
+    _check_device(logits, out, uniform, request, step, *(x for x in (temperature, top_k, top_p, min_p) if isinstance(x, torch.Tensor)))
     fn = _fn("sampling_filters", "tt_sample_filtered", "pliipfpipfpfpupppp")
     _check(fn(_ptr(logits), logits.stride(0), rows, vocab, settings[0][0], float(settings[0][1]), settings[1][0], int(settings[1][1]), settings[2][0],
               float(settings[2][1]), settings[3][0], float(settings[3][1]), _ptr(uniform), seed & ((1 << 64) - 1), _ptr(request), _ptr(step), _ptr(out),

@@ -337,10 +337,6 @@ class CausalAttention(Mixer):
         return ctx.workspace.get_zeroed("attention.tickets", (max(ctx.sequences * self.kv_heads, 64),), torch.int32)
 
     # ------------------------------------------------------------------ a cache in 4 bits
-    EXPAND_4BIT_FROM = 16           # new tokens a sequence (on average) from which a step's blocks are expanded
-    # Keys times tiles from which few long tiles are cut into even runs instead of 8 slices (heads of 128, slices against runs: one sequence
-    # of 16,384 tokens, 8 heads, 18 and 22 us, of 32,768 29 and 27; four of 16,384 33 and 28; two of up to 40,001 42 and 33).
-    EVEN_4BIT_FROM = 8 * 24576
     EXPAND_4BIT_BYTES = 4 << 30     # most scratch memory that the expanded blocks may take
 
     def span_4bit(self, ctx, width: int) -> int:
@@ -351,10 +347,21 @@ class CausalAttention(Mixer):
             return width
         return min(width, (ctx.n_tokens - ctx.sequences + 1 + bound - 1 + 62) // 64 + 1)
 
+    def keys_4bit(self, ctx) -> int:
+        """How many keys a token of the step sees at most."""
+        return min(ctx.max_total, self.window or self.chunk or ctx.max_total)
+
     def expands_4bit(self, ctx, width: int) -> bool:
         """Whether a step's prompts go through float16 copies of the blocks that they see: the 4-bit kernel reads a sequence's cache
-        once for every few tokens, the copies are read by the tcgen05 kernel, which takes many at a time."""
-        if ctx.decode or ctx.n_tokens < self.EXPAND_4BIT_FROM * ctx.sequences:
+        once for every 16 query rows, from as many CTAs as it takes; the copies, which have to be made, are read by the tcgen05 kernel once for every 128, by
+        one CTA after another.  Compared are nanoseconds a block of 64 tokens of the sequences, fitted to 1 to 16 sequences of 16 to 512 tokens
+        behind 1 to 24,000 (32/8 heads of 128 behind 8,000, copies not used and used: 64 tokens 63 and 132 us, 256 tokens 217 and 134; 16 sequences
+        behind 2,000: 16 tokens 62 and 88, 64 tokens 161 and 89)."""
+        if ctx.decode:
+            return False
+        tiles = ctx.n_tokens * self.heads / 16
+        copies = (540 + 3.8 * self.head_dim) * max(1.0, tiles / 8 / (1.5 * api.sm_count(ctx.status.device))) + ctx.sequences * self.kv_heads * self.head_dim / 13
+        if tiles * (1.2 + self.head_dim / 64) <= copies:
             return False
         return ctx.sequences * self.span_4bit(ctx, width) * 64 * self.kv_heads * self.head_dim * 4 <= self.EXPAND_4BIT_BYTES
 
@@ -372,18 +379,14 @@ class CausalAttention(Mixer):
             api.attention_half(q, keys, values, scales, marks, named, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
                                self.head_dim, self.scale, self.reach, mixed, ctx.status, sinks=self.sinks)
             return
-        group, sms = self.heads // self.kv_heads, api.sm_count(ctx.status.device)
-        wide = group > 8 or ctx.n_tokens > ctx.sequences               # tiles of up to 16 rows, of which an SM holds half as many
-        units = (ctx.sequences if ctx.decode else -(-ctx.n_tokens * group // 16)) * self.kv_heads
-        bound = min(ctx.max_total, self.window or self.chunk or ctx.max_total)
+        sms = api.sm_count(ctx.status.device.index)
+        splits = api.attention_4bit_splits(ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads, self.keys_4bit(ctx), sms)
         part_acc = part_ml = tickets = None
-        if units * 8 <= 2 * sms and bound >= 8192 and bound * units >= self.EVEN_4BIT_FROM:
-            splits, rows = 0, api.attention_4bit_part_rows(ctx.status.device)
+        if splits == 0:
+            rows = api.attention_4bit_part_rows(ctx.status.device)
             part_acc = ctx.scratch("attention.part_acc", (rows * self.head_dim,), torch.float32)
             part_ml = ctx.scratch("attention.part_ml", (rows * 2,), torch.float32)
             tickets = ctx.workspace.get_zeroed("attention.run_tickets", (4 * sms,), torch.int32)
-        else:       # slices of the keys until the CTAs fill the GPU once, each of 256 keys at least
-            splits = max(1, min((2 if wide else 4) * sms // max(1, units), bound // 256, 8))
         api.attention_4bit(q, cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, ctx.n_tokens, self.heads, self.kv_heads,
                            self.head_dim, self.scale, self.reach, splits, mixed, part_acc, part_ml, ctx.status, one_token_each=ctx.decode,
                            sinks=self.sinks, tickets=tickets)
