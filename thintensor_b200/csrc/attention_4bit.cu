@@ -866,24 +866,23 @@ cudaError_t launch_attention(const Attention4& a, cudaStream_t stream) {
 
 }  // namespace
 
-// one_token_each: n_tokens == sequences and every sequence brings one.  splits 1..8: slices of the keys (see above); 0: even runs, whose
+// rows: query rows of a tile at most, 4, 8 or 16.  one_token_each: n_tokens == sequences and every sequence brings one.  splits 1..8: slices of the keys (see above); 0: even runs, whose
 // parts need part_rows rows of head_dim numbers in part_acc and of 2 in part_ml, 2 for each row of a tile and each CTA that the device
 // holds, and a ticket for each of those CTAs, zero before the call and after it.
 extern "C" int tt_attention_4bit(const void* q, const void* k_pool, const void* v_pool, const int* table, int table_width, int pool_blocks,
                                  const int* cu, const int* len_before, int sequences, int n_tokens, int heads, int kv_heads, int head_dim,
-                                 float scale, int window, int splits, int one_token_each, int wide, void* out, float* part_acc, float* part_ml,
+                                 float scale, int window, int splits, int one_token_each, int rows, void* out, float* part_acc, float* part_ml,
                                  unsigned* tickets, long long part_rows, unsigned* status, const float* sinks, cudaStream_t stream) {
     if (n_tokens <= 0 || sequences <= 0) return 0;
     if (!cache4::takes(heads, kv_heads, head_dim) || splits < 0 || splits > 8 || !(scale > 0.0f) || (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)q) & 15) != 0 ||
-        (splits == 0 && (!part_acc || !part_ml || !tickets)))
+        (splits == 0 && (!part_acc || !part_ml || !tickets)) || (rows != 4 && rows != 8 && rows != 16) || heads / kv_heads > rows)
         return (int)cudaErrorInvalidValue;
-    const int group = heads / kv_heads;
     const Attention4 a{(const __nv_bfloat16*)q, (const uint8_t*)k_pool, (const uint8_t*)v_pool, table, table_width, pool_blocks, cu, len_before, sequences, n_tokens,
                        heads, kv_heads, scale * 1.4426950408889634f, window, splits, one_token_each, (__nv_bfloat16*)out, part_acc, part_ml, tickets, part_rows,
                        status, sinks};
 #define TT_LAUNCH_D(D)                                                                  \
-    if (group > 8 || wide) return (int)launch_attention<D, 2, false>(a, stream);       \
-    if (group > 4) return (int)launch_attention<D, 1, false>(a, stream);               \
+    if (rows == 16) return (int)launch_attention<D, 2, false>(a, stream);              \
+    if (rows == 8) return (int)launch_attention<D, 1, false>(a, stream);               \
     return (int)launch_attention<D, 1, true>(a, stream)
     switch (head_dim) {
         case 32: TT_LAUNCH_D(32);

@@ -1405,6 +1405,14 @@ def attention_4bit_part_rows(device: torch.device | int | None = None) -> int:
     return 64 * sm_count(device)
 
 
+def _rows_4bit(sequences: int, n_tokens: int, group: int) -> int:
+    """Query rows of a tile: as many as one token has, or a sequence's tokens in the mean (16 sequences of 2 tokens and 4 heads a key/value head, 2,011
+    cached tokens: in tiles of 4 rows 22 us, of 8 17, of 16 22; of 5 tokens: 43, 37 and 35)."""
+    if group > 8 or (n_tokens > sequences and n_tokens * group > 8 * sequences):
+        return 16
+    return 8 if group > 4 or n_tokens > sequences else 4
+
+
 @functools.lru_cache(maxsize=4096)
 def attention_4bit_splits(sequences: int, n_tokens: int, heads: int, kv_heads: int, longest: int, sms: int) -> int:
     """``splits`` for :func:`attention_4bit`, from a step's shape: ``longest`` is how many keys a token sees at most.  Slices in powers of two while all
@@ -1412,18 +1420,17 @@ def attention_4bit_splits(sequences: int, n_tokens: int, heads: int, kv_heads: i
     eight query rows, and half as many of the form with eight warps that the kernel takes while there is an SM for each CTA.  Even runs for long caches that
     would fill the GPU with less than its CTAs.  (440 shapes of 1 to 40 sequences, 1 to 24 tokens and 300 to 20,000 keys: 3.5 % above
     the fastest of 0 to 8 in the mean, 1.7 times at most.)"""
-    group = heads // kv_heads
-    wide = group > 8 or n_tokens > sequences
-    tokens = 1 if n_tokens == sequences else (16 if wide else 8) // group          # of a tile
+    rows = _rows_4bit(sequences, n_tokens, heads // kv_heads)
+    tokens = 1 if n_tokens == sequences else rows // (heads // kv_heads)           # of a tile
     tiles = sequences * -(-n_tokens // (sequences * tokens)) * kv_heads
     launched = tiles if n_tokens == sequences else (n_tokens // tokens + sequences) * kv_heads
-    if longest >= 8192 and longest * tiles >= 8 * 24576 and tiles <= (2 if wide else 4) * sms:
+    held = 2 if rows == 16 else 4                                       # CTAs of four warps on an SM
+    if longest >= 8192 and longest * tiles >= 8 * 24576 and tiles <= held * sms:
         return 0
     best = 1
     for splits in (2, 4, 8):
         single = launched * splits <= sms
-        held = (2 if wide else 4) // (2 if single else 1)
-        if longest // 256 >= splits and (launched if single else tiles) <= max(1, sms // 18) * (18 * held // splits):
+        if longest // 256 >= splits and (launched if single else tiles) <= max(1, sms // 18) * (18 * (held // 2 if single else held) // splits):
             best = splits
     return best
 
@@ -1466,11 +1473,10 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
             _need_aligned(t, name)
         if tickets is None or tickets.dtype != torch.int32 or tickets.numel() < 4 * sm_count(q.device):
             raise KernelError(f"attention_4bit: even runs need {4 * sm_count(q.device)} int32 tickets")
-    wide = not one_token_each and n_tokens > sequences                 # several tokens of a sequence share a pass over its keys
     _check_device(q, k_pool, v_pool, table, cu, len_before, out, part_acc, part_ml, tickets, sinks, status)
     fn = _fn("attention_4bit", "tt_attention_4bit", "ppppiippiiiiifiiiipppplppp")
     _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(table), width, blocks, _ptr(cu), _ptr(len_before), sequences, n_tokens,
-              heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, 1 if wide else 0, _ptr(out), _ptr(part_acc), _ptr(part_ml),
+              heads, kv_heads, head_dim, scale, window, splits, 1 if one_token_each else 0, _rows_4bit(sequences, n_tokens, heads // kv_heads), _ptr(out), _ptr(part_acc), _ptr(part_ml),
               _ptr(tickets), rows, _ptr(status), _ptr(sinks), _stream()), "attention_4bit")
 
 

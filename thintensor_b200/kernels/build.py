@@ -43,7 +43,7 @@ SOURCES: dict[str, list[str]] = {
     "attention_mma": [],
     "attention_tcgen05": [],
     "cache_4bit": [],
-    "attention_4bit": ["--split-compile=0"],
+    "attention_4bit": [],
     "recurrent": [],
     "recurrent_chunks": [],
     "latent_attention": [],
