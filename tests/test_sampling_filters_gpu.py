@@ -65,6 +65,32 @@ def test_settings_of_every_rows_own():
             min_p=pick([0.0, 0.03, 0.3], torch.float32))
 
 
+@pytest.mark.parametrize("vocab", [5, 700, 6001])
+@pytest.mark.parametrize("temperature", [1e-3, 0.4, 1.6])
+def test_a_nucleus_of_few_tokens(vocab, temperature):
+    """Weights that stand out of what is left, whose sums come close to the share: within the error of a float32 sum of all weights, and further off."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = 9
+    weights = torch.tensor([8.0, 4.0, 2.0, 1.0, 1.0], dtype=torch.float64)          # their running sums are 1/2, 3/4, 7/8 of the whole
+    x = torch.full((rows, vocab), -math.inf)
+    for i in range(rows):
+        x[i, torch.randperm(vocab, generator=g)[:5]] = (temperature * weights.log()).float()
+    if vocab > 5:
+        x[::3] = torch.maximum(x[::3], temperature * (-17.0 + 0.5 * torch.randn(rows // 3, vocab, generator=g)))      # a little weight beside them
+    u = torch.rand(rows, generator=g)
+    for top_p in (0.3, 0.4999, 0.5001, 0.749, 0.7499, 0.7501, 0.8749, 0.8751, 0.9999):
+        for min_p in (0.0, 0.07, 0.2, 0.3, 0.7):
+            compare(x, u, temperature=temperature, top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("min_p", [0.0, 1e-6, 0.001, 0.05, 0.4])
+@pytest.mark.parametrize("top_p", [0.05, 0.6, 0.97, 1.0])
+def test_min_p_and_a_nucleus(top_p, min_p):
+    """From rows whose nucleus is a handful to rows where half the vocabulary is above min-p (more than are compared with each other)."""
+    for spread, temperature in ((0.1, 1.0), (1.0, 0.5), (2.5, 0.8), (6.0, 1.0)):
+        compare(*logits_of(2, 30011, seed=int(10 * spread), spread=spread), temperature=temperature, top_p=top_p, min_p=min_p)
+
+
 @pytest.mark.parametrize("settings", [dict(temperature=1.0, top_k=3), dict(temperature=1.0, top_p=0.5), dict(temperature=1.0, min_p=0.5), dict(temperature=0.0),
                                       dict(temperature=1.0, top_k=300), dict(temperature=1.0)])
 @pytest.mark.parametrize("vocab", [64, 3000, 40000])
