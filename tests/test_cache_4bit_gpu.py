@@ -809,3 +809,49 @@ def test_the_command_line_keeps_4_bits(tmp_path, capsys):
     assert json.loads(capsys.readouterr().out.strip().splitlines()[-1])["modes"]["whole"]["cosine_similarity"] > 0.99
     assert cli.main(["run", str(tmp_path), "--prompt-token-ids", "1,2", "--cache", "4bit", "--dtype", "fp32"]) == 2
     assert "4 bits" in capsys.readouterr().err
+
+
+def test_even_runs_on_two_streams_at_once_with_scratch_of_their_own():
+    steps = [Step([9000], [1], 2, 64, seed=1), Step([3000, 7000], [1, 1], 2, 64, seed=2)]
+    inputs = [queries(step, 8) for step in steps]
+    scratch = [part_scratch(64) for _ in steps]
+    want = [run_attention(step, q, 8, splits=0, one=True).clone() for step, q in zip(steps, inputs)]
+    outs = [torch.full_like(w, 7.0) for w in want]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                run_attention(steps[i], inputs[i], 8, splits=0, one=True, scratch=scratch[i], out=outs[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and not any(s["tickets"].any() for s in scratch)
+
+
+def test_the_same_scratch_for_steps_of_other_shapes():
+    """A layer's workspace serves prompts and decoding in turn, captured steps among them."""
+    mixers = []
+    for before, new in (([170, 90], [40, 60]), ([9000], [1]), ([64] * 3, [30, 2, 1])):
+        step = Step(before, new, 2, 64)
+        mixer, ctx, cache = layer(step, 8, all(n == 1 for n in new))
+        mixers.append((step, mixer, ctx, cache, queries(step, 8)))
+    shared = mixers[0][2].workspace
+    graphs = []
+    for copies in (True, False):
+        for step, mixer, ctx, cache, q in mixers:
+            ctx.workspace = shared
+            if not ctx.decode:
+                mixer.expands_4bit = lambda ctx, width: copies  # noqa: B023
+            out = torch.full_like(q, 7.0)
+            mixer.attend(ctx, q, cache, step.table, out)
+    for copies in (True, False):
+        for step, mixer, ctx, cache, q in mixers:
+            if not ctx.decode:
+                mixer.expands_4bit = lambda ctx, width: copies  # noqa: B023
+            out, graph = torch.full_like(q, 7.0), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                mixer.attend(ctx, q, cache, step.table, out)
+            graphs.append((graph, out, step, q, copies and not ctx.decode))
+    for graph, out, step, q, copies in graphs + graphs[::-1]:
+        out.fill_(7.0)
+        graph.replay()
+        (close_to_half if copies else close_to)(out, step, q, 8)

@@ -1446,7 +1446,7 @@ def attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     anew: prompts are faster through :func:`expand_4bit`.  ``splits`` 1 to 8 cuts the keys of a sequence into so many slices; 0 gives every
     CTA that the device holds an equal run of all sequences' blocks, whose parts need the float32 scratch ``part_acc``
     [:func:`attention_4bit_part_rows` * head_dim] and ``part_ml`` [the same * 2], and ``tickets``: int32, four for each multiprocessor, zero before the
-    call and after it."""
+    call and after it; all three belong to one call at a time (calls on two streams bring their own)."""
     if not cache_4bit_supports(q.dtype, heads, kv_heads, head_dim):
         raise KernelError(f"attention over 4 bits takes bfloat16, head sizes {CACHE_4BIT_DIMS} and up to 16 query heads per key/value head, not {q.dtype}, "
                           f"{heads}/{kv_heads} heads of {head_dim}")
