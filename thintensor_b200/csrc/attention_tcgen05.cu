@@ -470,7 +470,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             float mx = fmaxf(max3(mxa, mxb, mxc), mxd);
             if (SPLIT == 2) {
                 pair_max[i & 1][half][r] = mx;
+                // with P over the scores, a warp stores over what its partner has read: the partner's loads come before the barrier, its stores after it
+                if (L::P_OVER_S) fence_before_sync();
                 pair_barrier();
+                if (L::P_OVER_S) fence_after_sync();
                 mx = fmaxf(mx, pair_max[i & 1][half ^ 1][r]);
             }
             // HALF: the largest weight in use is 2^7 when its scale is new and never more than 2^15, float16's reach, however large the scores are (so
