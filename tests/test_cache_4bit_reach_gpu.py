@@ -9,11 +9,99 @@ import math
 import pytest
 import torch
 
-from test_cache_4bit_gpu import Step, queries
+import plain_cache_4bit as plain
+from test_cache_4bit_gpu import Step, queries, run_attention
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+
+
+def rewrite(step, name):
+    """The pool's bytes from the codes, scales and least values as they now are."""
+    n, s, m = getattr(step.cache, name + "_parts")
+    setattr(step.cache, name + "_host", torch.stack([torch.stack([plain.write_block(n[i, h], s[i, h], m[i, h], name == "v") for h in range(step.kv)])
+                                                     for i in range(n.shape[0])]))
+    step.k_pool, step.v_pool = step.cache.pools()
+
+
+def enlarge(step, name, b, token, factor):
+    """All heads' numbers of one token times a power of two."""
+    _, s, m = getattr(step.cache, name + "_parts")
+    block, at = int(step.cache.table[b, token // 64]), token % 64
+    s[block, :, at] *= factor
+    m[block, :, at] *= factor
+    rewrite(step, name)
+
+
+def turn_away(step, b, token, size):
+    """The token's keys are -size in every number: queries of positive numbers hardly weigh it."""
+    n, s, m = step.cache.k_parts
+    block, at = int(step.cache.table[b, token // 64]), token % 64
+    n[block, :, at], s[block, :, at], m[block, :, at] = 0, 1.0, -size
+    rewrite(step, "k")
+
+
+def close_to_own(got, step, q, heads, window=0, copied=False):
+    """Every row by what it sees itself.  A score is off by `moved` of the magnitudes that it is added up from, its weight by twice that of itself (the maximum moves
+    as well), and so every key counts by its own weight in the output's sum and in the sum of weights.
+
+    Over 4 bits: scores within 160 float32 roundings and 2^-20; weights 2^-11, and a weight under float16's 2^-14 by 2^-25, 2^-39 of the row's largest weight
+    times scale.  Over copies: keys 2^-11 of themselves and 2^-24 of their token's largest number (float16's smallest step beside a largest number of at least 2^-1),
+    float32 sums 2^-16; weights, values and the sum 2^-11 each; a weight under 2^-14 by 2^-25 times a value of at most 2^15, where the row's largest weight is at least 2^7 and
+    that token's largest number at least 2^-1: 2^-16 of the largest product.  The output 2^-8."""
+    rows, scale = q.double().cpu().view(-1, heads, step.dim), step.dim ** -0.5
+    got, at = got.double().cpu().view_as(rows), 0
+    for b, (have, count) in enumerate(zip(step.before, step.new)):
+        for h in range(heads):
+            kh = h // (heads // step.kv)
+            wide = lambda t: t.double().repeat_interleave(32, dim=-1)  # noqa: E731
+            k, kn, ks, km = step.cache.rows("k", b, kh, have + count)
+            v, vn, vs, vm = step.cache.rows("v", b, kh, have + count)
+            k_size, v_size = wide(ks) * kn + wide(km).abs(), wide(vs) * vn + wide(vm).abs()
+            for j in range(count):
+                seen, row = slice(plain.first_key(have + j, window), have + j + 1), rows[at + j, h]
+                p = torch.softmax((k[seen] @ row) * scale, 0)
+                want, weight = p @ v[seen], p @ v_size[seen]
+                reach = (k_size[seen] @ row.abs()) * scale
+                if copied:
+                    moved = (2.0 ** -11 + 2.0 ** -16) * reach + 2.0 ** -24 * k[seen].abs().amax(1) * row.abs().sum() * scale
+                    least, fixed = 2.0 ** -16 * (p * v[seen].abs().amax(1)).max(), 3 * 2.0 ** -11
+                else:
+                    moved = 160 * 2.0 ** -24 * reach + 2.0 ** -20
+                    least, fixed = 2.0 ** -39 * 16 * (p * vs[seen].amax(1)).max(), 2.0 ** -11
+                off = p * torch.expm1((2 * moved).clamp_max(500.0))
+                allowed = 2.0 ** -8 * want.abs() + fixed * weight + off @ v_size[seen] + off.sum() * weight + len(p) * least
+                found = (got[at + j, h] - want).abs()
+                assert bool((found <= allowed + 1e-30).all()), (b, h, j, float((found / (allowed + 1e-30)).max()))
+        at += count
+    assert int(step.status.item()) == 0
+
+
+# -------------------------------------------------------------------------------------------- attention over 4 bits
+@pytest.mark.parametrize("dim,kv,heads", [(32, 2, 2), (64, 2, 8), (96, 1, 8), (128, 2, 10), (128, 1, 16)])
+@pytest.mark.parametrize("token", [62, 66, 70])                         # in the block of what the rows before it see, and in the next one
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 34, 2.0 ** 100])
+@pytest.mark.parametrize("splits", [1, 2, 0])
+def test_a_value_that_later_tokens_alone_see(dim, kv, heads, token, factor, splits):
+    step = Step([60, 5], [12, 3], kv, dim, seed=dim + heads)
+    enlarge(step, "v", 0, token, factor)
+    q = queries(step, heads)
+    close_to_own(run_attention(step, q, heads, splits=splits), step, q, heads)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("group", [1, 4, 16])
+@pytest.mark.parametrize("token", [3, 199, 140])
+@pytest.mark.parametrize("factor", [2.0 ** 40, 2.0 ** 70, 2.0 ** 110])
+@pytest.mark.parametrize("splits", [1, 3, 0])
+def test_a_value_of_little_weight(dim, group, token, factor, splits):
+    """Weights of e^-100 to e^-400 beside values of 2^40 to 2^110."""
+    step = Step([200, 90], [1, 1], 2, dim, seed=dim)
+    turn_away(step, 0, token, 32.0)
+    enlarge(step, "v", 0, token, factor)
+    q = queries(step, 2 * group).abs()
+    close_to_own(run_attention(step, q, 2 * group, splits=splits, one=True), step, q, 2 * group)
 
 
 # ----------------------------------------------------------------------------------------------- prompts over copies

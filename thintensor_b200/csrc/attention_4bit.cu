@@ -12,9 +12,11 @@
 //
 // Queries are float16 after a power of two that brings a row's greatest number to 2^14: exact but for what lies 2^-28 below that.
 // The weights p s' are rounded to float16 (11 bits): with weights in bfloat16 the two terms of out, which are of opposite sign and
-// each several times their sum, were off by 0.4 % of it.  So that float16 holds them whatever the values' size, p is formed relative to
-// the running maximum times 2^(E - 14), E the exponent of the largest scale that the warp has met (at least -40): the weights stay
-// below 2^15, and what falls under 2^-14 is less than 2^-29 of the largest.  The second term takes p in two bfloat16 parts (16 bits)
+// each several times their sum, were off by 0.4 % of it.  So that float16 holds them whatever the values' size, the running maximum is
+// one of score + E - 14 in log2 units, E the exponent of the largest of the key's value scales (at least -40), and p is relative to it: a row's weights
+// stay below 2^15, its largest is 2^14 or more, and what falls under 2^-14, float16's last full number, is less than 2^-28 of that.  A row's unit so
+// depends on what it sees, and by how much it weighs it, alone (with the largest scale that the warp had met as the unit, a value of 2^34 that later
+// tokens alone see, or of little weight, left the others no bits).  The second term takes p in two bfloat16 parts (16 bits)
 // and m' as it is, the second term of S the queries' sums in three.  All sums are float32.
 //
 // Rows of up to four queries (DUP) stand twice in the tile's eight columns, which would otherwise be half empty: the weights of one
@@ -61,6 +63,11 @@ __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint3
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // two float32 numbers at a time
+__device__ __forceinline__ void fma_two_up(float& a, float& b, float x0, float x1, float y0, float y1, float z) {
+    asm("{\n\t.reg .b64 x, y, z, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %6};\n\t"
+        "fma.rp.f32x2 d, x, y, z;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(a), "=f"(b) : "f"(x0), "f"(x1), "f"(y0), "f"(y1), "f"(z));
+}
 __device__ __forceinline__ void fma_two(float& a, float& b, float x0, float x1, float y0, float y1, float z0, float z1) {
     asm("{\n\t.reg .b64 x, y, z, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
         "fma.rn.f32x2 d, x, y, z;\n\tmov.b64 {%0, %1}, d;\n\t}"
@@ -118,8 +125,7 @@ template <int D, int NQ, bool DUP> struct Rows4 {
     float o[2 * G][NQ][4];              // [0], [1]: number 16 dt + r, queries 8 nq + 2 c + e; [2], [3]: number + 8, sixteenfold
     float least[NQ][4];                 // row r = group r: the least values' share
     float scale[NQ][2];                 // of the scores of queries 8 nq + 2 c + e, in log2 units
-    float m_run[NQ][2], l_run[NQ][2];   // l: this lane's share (its keys) until the end
-    int e_run;                          // E: all weights and sums are relative to 2^(m_run + E - 14)
+    float m_run[NQ][2], l_run[NQ][2];   // the maximum of score + E - 14, to whose power of two all weights and sums are relative; l: this lane's share (its keys) until the end
     int pos[NQ][2], first[NQ][2];       // queries 8 nq + 2 c + e see keys first .. pos
 };
 
@@ -165,49 +171,68 @@ __device__ __forceinline__ void scores_of_block(const Rows4<D, NQ, DUP>& st, con
     }
 }
 
+// E - 14 of two neighbouring tokens as a pair of bfloat16 numbers: E the exponent of a token's largest scale, at least -40 (positive bfloat16 numbers
+// order like their bits; a scale that is not a number counts for nothing here).
+template <int G>
+__device__ __forceinline__ uint32_t exponents_of(const uint8_t* __restrict__ two_tokens) {
+    uint32_t w[G];                                                     // G scales of the first token, then those of the second
+    load_words<G>(two_tokens, w);
+    auto larger = [](uint32_t a, uint32_t b) {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    };
+    uint32_t most;                                                     // the first token's largest scale in the low half, the second's in the high one
+    if constexpr (G == 1) most = w[0];
+    else if constexpr (G == 2) most = larger(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632));
+    else if constexpr (G == 3) most = larger(larger(__byte_perm(w[0], w[1], 0x7610), __byte_perm(w[0], w[2], 0x5432)), __byte_perm(w[1], w[2], 0x7610));
+    else {
+        const uint32_t a = larger(w[0], w[1]), b = larger(w[2], w[3]);
+        most = larger(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+    }
+    const uint32_t lo = most & 0xffffu, hi = most >> 16;
+    const int first = lo <= 0x7f80u ? (int)(lo >> 7) - 127 : -127, second = hi <= 0x7f80u ? (int)(hi >> 7) - 127 : -127;
+    return pack_bf16((float)(max(first, -40) - 14), (float)(max(second, -40) - 14));       // whole numbers below 256: exact
+}
+
 // Their running softmax and what its weights make of the block's values.  MASKED: some query does not see some key of the block.
 template <int D, int NQ, bool DUP, bool MASKED>
 __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uint8_t* __restrict__ vb, float (&s)[4][NQ][4], int key_base,
-                                                int first_seen, int last_pos, int r, int c) {
+                                                int last_pos, int r, int c) {
     constexpr int G = Rows4<D, NQ, DUP>::G;
     const int lane = 4 * r + c, token0 = token_of_row(r);
     const uint8_t* scales = vb + code_bytes(D);
     const uint8_t* mins = scales + 2 * TT_BLOCK_TOKENS * G;
-    // the bits of the block's largest scale: a lane looks at two neighbouring tokens (positive bfloat16 numbers order like their bits; a scale
-    // that is not a number counts for nothing here)
-    uint32_t top = 0u;
-    {
-        uint32_t two[G];
-        load_words<G>(scales + 2 * lane * 2 * G, two);
-        if constexpr (!MASKED) {
-            __nv_bfloat162 most = *reinterpret_cast<const __nv_bfloat162*>(&two[0]);
+    if constexpr (MASKED) {
 #pragma unroll
-            for (int i = 1; i < G; ++i) most = __hmax2(most, *reinterpret_cast<const __nv_bfloat162*>(&two[i]));
-            const uint32_t bits = *reinterpret_cast<const uint32_t*>(&most), lo = bits & 0xffffu, hi = bits >> 16;
-            top = max(lo <= 0x7f80u ? lo : 0u, hi <= 0x7f80u ? hi : 0u);
-        } else {
+        for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int i = 0; i < 2 * G; ++i) {
-                const uint32_t bits = (two[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                const int key = key_base + 2 * lane + i / G;
-                if (bits <= 0x7f80u && key <= last_pos && key >= first_seen) top = max(top, bits);
+            for (int hi = 0; hi < 2; ++hi) {
+                const int key = key_base + 16 * kt + token0 + 2 * hi;
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (!(key <= st.pos[nq][e] && key >= st.first[nq][e])) s[kt][nq][2 * hi + e] = -INFINITY;
             }
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                for (int hi = 0; hi < 2; ++hi) {
-                    const int key = key_base + 16 * kt + token0 + 2 * hi;
-#pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (!(key <= st.pos[nq][e] && key >= st.first[nq][e])) s[kt][nq][2 * hi + e] = -INFINITY;
-                }
-        }
     }
-    const int e_new = max(st.e_run, (int)(__reduce_max_sync(0xffffffffu, top) >> 7) - 127);
-    const float e_old = (float)(st.e_run - 14), e_now = (float)(e_new - 14);
-    st.e_run = e_new;
+    const uint32_t exponents = exponents_of<G>(scales + 2 * lane * 2 * G);         // of tokens 2 lane and 2 lane + 1
+    float most[NQ][2];
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) most[nq][0] = most[nq][1] = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+            const uint32_t two = __shfl_sync(0xffffffffu, exponents, 8 * kt + 2 * (r >> 1) + hi);
+            const float unit = __uint_as_float(r & 1 ? two & 0xffff0000u : two << 16);
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) {                          // the scale is positive; rounded up, so that no weight leaves float16's reach
+                float x, y;
+                fma_two_up(x, y, s[kt][nq][2 * hi], s[kt][nq][2 * hi + 1], st.scale[nq][0], st.scale[nq][1], unit);
+                most[nq][0] = fmaxf(most[nq][0], x);
+                most[nq][1] = fmaxf(most[nq][1], y);
+            }
+        }
     float corr[NQ][2];
     bool grew = false;
 #pragma unroll
@@ -215,16 +240,14 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
         float base[2], sum[2] = {0.0f, 0.0f}, m_new[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(s[kt][nq][e], s[kt][nq][2 + e]));
+            float mx = most[nq][e];
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            m_new[e] = fmaxf(st.m_run[nq][e], __fmul_ru(mx, st.scale[nq][e]));   // the scale is positive; rounded up, so that no weight leaves float16's reach
-            corr[nq][e] = m_new[e] == -INFINITY ? 1.0f : fast_exp2((st.m_run[nq][e] - m_new[e]) + (e_old - e_now));
+            m_new[e] = fmaxf(st.m_run[nq][e], mx);
+            corr[nq][e] = m_new[e] == -INFINITY ? 1.0f : fast_exp2(st.m_run[nq][e] - m_new[e]);
             grew = grew || corr[nq][e] != 1.0f;
-            base[e] = m_new[e] == -INFINITY ? 0.0f : -__fadd_ru(m_new[e], e_now);
+            base[e] = m_new[e] == -INFINITY ? 0.0f : -m_new[e];
         }
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -550,7 +573,6 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
     }
 
     Rows4<D, NQ, DUP> st;
-    st.e_run = -40;
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
         uint32_t most = 0u;                                            // bits of the row's greatest number without its sign
@@ -630,8 +652,8 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
         if (usable) {
             const int key_base = (begin + warp + i * WARPS) * TT_BLOCK_TOKENS;
             const bool all_visible = key_base + TT_BLOCK_TOKENS - 1 <= pos0 && key_base >= last_first;
-            if (all_visible) values_of_block<D, NQ, DUP, false>(st, value_ring, s, key_base, first_key, last_pos, r, c);
-            else values_of_block<D, NQ, DUP, true>(st, value_ring, s, key_base, first_key, last_pos, r, c);
+            if (all_visible) values_of_block<D, NQ, DUP, false>(st, value_ring, s, key_base, last_pos, r, c);
+            else values_of_block<D, NQ, DUP, true>(st, value_ring, s, key_base, last_pos, r, c);
         }
         __syncwarp();
         if (i + 1 < n_mine) fetch(v_pool, value_ring, &values_landed[warp], i + 1);
@@ -676,7 +698,7 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             for (int dt = 0; dt < 2 * G; ++dt)
                 if (!DUP || ((dt >> 1) & 1) == (c >> 1)) { dst[16 * dt] = st.o[dt][nq][e]; dst[16 * dt + 8] = st.o[dt][nq][2 + e]; }
             if (r == 0 && (!DUP || c < 2)) {
-                sh_m[warp * COLS + col] = __fadd_ru(st.m_run[nq][e], (float)(st.e_run - 14));
+                sh_m[warp * COLS + col] = st.m_run[nq][e];
                 sh_l[warp * COLS + col] = st.l_run[nq][e];
             }
         }
