@@ -127,6 +127,97 @@ def run_prompt(step, q, heads, window=0):
     return out
 
 
+@pytest.mark.parametrize("dim,kv,heads", [(32, 2, 2), (64, 2, 8), (96, 1, 8), (128, 2, 10), (128, 1, 16)])
+@pytest.mark.parametrize("token", [62, 66, 85])
+@pytest.mark.parametrize("factor", [2.0 ** 12, 2.0 ** 20, 2.0 ** 34, 2.0 ** 100])
+@pytest.mark.parametrize("names", ["v", "k", "kv"])
+def test_prompts_and_what_later_tokens_alone_see(dim, kv, heads, token, factor, names):
+    step = Step([60, 5], [30, 20], kv, dim, seed=dim + heads)
+    for name in names:
+        enlarge(step, name, 0, token, factor)
+    q = queries(step, heads)
+    close_to_own(run_prompt(step, q, heads), step, q, heads, copied=True)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("group", [1, 6])
+@pytest.mark.parametrize("token", [3, 140, 199])
+@pytest.mark.parametrize("factor", [2.0 ** 40, 2.0 ** 70, 2.0 ** 110])
+def test_prompts_and_a_value_of_little_weight(dim, group, token, factor):
+    step = Step([200, 90], [24, 3], 2, dim, seed=dim)
+    turn_away(step, 0, token, 32.0)
+    enlarge(step, "v", 0, token, factor)
+    q = queries(step, 2 * group).abs()
+    close_to_own(run_prompt(step, q, 2 * group), step, q, 2 * group, copied=True)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("names", ["v", "k", "kv"])
+@pytest.mark.parametrize("shrunk", [1.0, 2.0 ** -30])
+def test_prompts_with_a_large_token_beside_one_that_is_no_number(dim, names, shrunk):
+    """The block's tokens have powers of two of their own and groups that are not numbers at once; where the token that is none is itself small, too."""
+    step = Step([60], [30], 2, dim, seed=dim)
+    for name in names:
+        enlarge(step, name, 0, 85, 2.0 ** 34)
+        if shrunk != 1.0:
+            enlarge(step, name, 0, 75, shrunk)
+    step.cache.poison("v", 0, 75, 1, 0)
+    step.k_pool, step.v_pool = step.cache.pools()
+    heads = 8
+    q = queries(step, heads)
+    got = run_prompt(step, q, heads).view(30, heads, dim)
+    small = dim > 32 and "k" in names                                  # a small token then is not a number as a whole
+    for j in range(30):
+        seen = 60 + j >= 75
+        bad = torch.isnan(got[j])
+        assert bool(bad[4:, :32].all()) == seen and not bool(bad[:4].any())
+        assert bool(bad[4:].any()) == seen
+        assert bool(bad[4:, 32:].all()) == seen if small else not bool(bad[4:, 32:].any())
+    clean = Step([60], [15], 2, dim, seed=dim)
+    clean.cache = step.cache
+    close_to_own(got[:15].reshape(15, -1), clean, q[:15], heads, copied=True)
+
+
+@pytest.mark.parametrize("dim", [32, 96, 128])
+@pytest.mark.parametrize("factors", [dict(k=2.0 ** 9), dict(v=2.0 ** 9), dict(k=2.0 ** 40, v=2.0 ** 12), dict(k=2.0 ** -30), dict(v=2.0 ** -120), dict(k=2.0 ** 60, v=2.0 ** 60)])
+@pytest.mark.parametrize("bad", [False, True])
+def test_reading_back_blocks_of_unlike_tokens(dim, factors, bad):
+    """float16 times the block's power of two and 2^-8 for each step of the token; the marks' two readings as documented."""
+    step = Step([100], [3], 2, dim, seed=3)
+    for name, factor in factors.items():
+        enlarge(step, name, 0, 70, factor)
+        enlarge(step, name, 0, 102, 0.0)
+    if bad:
+        step.cache.poison("v", 0, 80, 1, dim // 32 - 1)
+        step.k_pool, step.v_pool = step.cache.pools()
+    keys, values, scales, marks, named = copies(step)
+    for w in (0, 1):
+        place, block, upto = int(named[0, w]), int(step.cache.table[0, w]), min(64, 103 - 64 * w)
+        for h in range(2):
+            k_scale, v_scale, byte = float(scales[0, place, h]), float(scales[1, place, h]), marks[place, h].cpu().long()
+            low, high = (byte & 15, byte >> 4) if k_scale < 0 or v_scale < 0 else (torch.zeros(64, dtype=torch.long),) * 2
+            if k_scale < 0:
+                none = high == 15
+                mask, k_step, v_step = torch.where(none, low, 0), torch.where(none, 0, low), torch.where(none, 0, high)
+            else:
+                mask, k_step, v_step = low, torch.zeros_like(low), high
+            for name, got, scale, steps in (("k", keys[place, h], k_scale, k_step), ("v", values[place, h].T, v_scale, v_step)):
+                n, s, m = (t[block, h] for t in getattr(step.cache, name + "_parts"))
+                want = plain.numbers(n, s, m)[:upto]
+                gone = torch.isnan(want)
+                whole = (k_scale < 0) & (mask[:upto] == 15)            # a small token with a group that is no number
+                if name == "v":
+                    assert bool((gone.any(1) | ~whole).all())
+                    marked = torch.stack([(mask[:upto] >> g & 1).bool() for g in range(dim // 32)], 1)
+                    assert torch.equal(marked, gone[:, ::32] | whole[:, None])
+                gone = gone | whole[:, None]
+                off = (got.double().cpu()[:upto] * (abs(scale) * 2.0 ** (-8.0 * steps[:upto].double()))[:, None] - want).abs()
+                largest = want.nan_to_num(0.0).abs().amax(1, keepdim=True)
+                assert bool(((off <= (2.0 ** -11 + 2.0 ** -23) * want.abs() + 2.0 ** -24 * largest + 1e-45) | gone).all())
+                assert bool((got.cpu()[upto:] == 0).all())
+    assert int(step.status.item()) == 0
+
+
 @pytest.mark.parametrize("dim", [32, 64, 96, 128])
 def test_prompts_give_the_same_bits_every_time(dim):
     """More tiles than the GPU holds at once, two of them on an SM, whose warps store weights over each other's scores."""

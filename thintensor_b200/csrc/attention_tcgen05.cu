@@ -28,7 +28,9 @@
 // The HALF instances read what expand_4bit_kernel made of a 4-bit cache: keys and values in float16 with a power of two a block and head, since a
 // number of such a cache is a sum that bfloat16 would round once more (the outputs' error against 64 bits: 0.0039 with bfloat16 blocks and weights,
 // 0.0017 with these, which is the rounding of the outputs).  The softmax threads bring their rows of queries to float16 in place, with a power of two
-// a row, before the first product; the weights are float16 too.
+// a row, before the first product; the weights are float16 too.  A weight carries its values' power of two: the maximum of a row is one of score + that
+// exponent, so the row's unit depends on what it sees and by how much it weighs it, and on nothing else in the tile (with the largest exponent of the tile's
+// blocks as the unit, a value of 2^34 that later tokens alone see left earlier rows no bits).  The sum of the weights without it, l, is kept beside them.
 //
 // The reference has no counterpart: it feeds prompts token by token through its
 // single-token attention (thinruntime/cli.py:2802-2807, thinruntime/triton_kernels.py:14-109).
@@ -125,9 +127,9 @@ struct Args {
     const float* gate;
     int gate_splits, gate_row, gate_per_head;
     long long gate_split_stride;
-    // the HALF instances only: float32 powers of two that a block's numbers are to be multiplied by, [keys or values][pool_blocks][kv_heads], and the
-    // numbers of a head (HD, or fewer: the rest of a row is read as zeros, or not used).  A values' scale below zero: groups of 32 numbers of some tokens
-    // are NaN and read as zeros, block_marks [pool_blocks][kv_heads][64] has a bit for each
+    // the HALF instances only: float32 powers of two that a block's numbers are to be multiplied by, [keys or values][pool_blocks][kv_heads], whose signs
+    // say whether block_marks [pool_blocks][kv_heads][64] has anything to add (see cache_4bit.cuh), and the numbers of a head (HD, or fewer: the rest of a
+    // row is read as zeros, or not used)
     const float* block_scales;
     const uint8_t* block_marks;
     int dim;
@@ -324,8 +326,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         auto pair_barrier = [&]() { if (SPLIT == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
         auto expired = [&]() { if (lane == 0) atomicOr(args.status, TT_STATUS_WAIT_EXPIRED); ok = false; };
         const int* table_row = args.table + (size_t)b * args.table_width;
-        float row_scale = 1.0f, value_scale = 1.0f, next_key = 1.0f, next_value = 1.0f;
+        float row_scale = 1.0f, next_key = 1.0f, next_value = 1.0f;
         int this_block = 0, next_block = 0;
+        float unit = 0.0f;                                        // HALF: l is relative to 2^(m_used - unit), O to 2^m_used
         unsigned not_numbers = 0;                                 // groups of 32 numbers of the row's output
         // a block outside the pool is read as block 0 (and flagged) by the thread that loads it
         auto scales_at = [&](int i) {
@@ -338,10 +341,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             next_key = __ldg(args.block_scales + this_block);
             next_value = __ldg(value_scales + this_block);
             next_block = scales_at(1);
-            // O is in units of the largest scale of the values that the tile sees
-            value_scale = 0.0f;
-            for (int i = lane; i < n_blocks; i += 32) value_scale = fmaxf(value_scale, fabsf(__ldg(value_scales + scales_at(i))));
-            value_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(value_scale)));
             // 64 numbers of the row's queries a thread, 16 bytes a time, each thread from another bank
             if (!mbar_wait(smem_u32(&q_full), 0)) expired();
             uint8_t* row = q_smem + half * ROWS * 128 + r * 128;
@@ -373,15 +372,18 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0 && ok) mbar_arrive(smem_u32(&q_ready));
         }
         for (int i = 0; i < n_blocks; ++i) {
-            float value_part = 1.0f;
+            float value_exponent = 0.0f;
+            int unlike = -1;                                      // a block whose tokens have powers of two of their own (the same for the whole warp)
             if constexpr (HALF) {
                 // neither infinite nor zero, so that a masked score stays what it is (scores of that size are infinite or zero themselves)
-                scale_log2 = fminf(fmaxf(row_scale * next_key, 1e-36f), 1e36f);
-                value_part = __fdividef(fabsf(next_value), value_scale);  // powers of two, at most one
-                if (next_value < 0.0f) {
+                scale_log2 = fminf(fmaxf(row_scale * fabsf(next_key), 1e-36f), 1e36f);
+                value_exponent = (float)((int)((__float_as_uint(next_value) >> 23) & 255u) - 127);
+                if (next_key < 0.0f || next_value < 0.0f) {
                     const uint8_t* marks = args.block_marks + (size_t)this_block * KEYS;
                     const int key0 = (block0 + i) * KEYS;
-                    for (int j = max(0, first - key0); j < KEYS && key0 + j <= pos; ++j) not_numbers |= marks[j];
+                    if (next_value < 0.0f)
+                        for (int j = max(0, first - key0); j < KEYS && key0 + j <= pos; ++j) not_numbers |= cache4::marked_groups(marks[j], next_key < 0.0f);
+                    if (next_key < 0.0f || __any_sync(0xffffffffu, (marks[lane] | marks[lane + 32]) & 0xf0)) unlike = this_block;
                 }
                 this_block = next_block;
                 next_key = __ldg(args.block_scales + next_block);
@@ -401,6 +403,17 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int c = 0; c < HALF_KEYS / 32; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) s[32 * c + j] = tmem_loaded(raw[c][j]);
+            }
+            if (HALF && unlike >= 0) {                                // rare: scores in log2 units, and with the tokens' steps below their block's value exponent
+                const uint8_t* marks = args.block_marks + (size_t)unlike * KEYS + half * HALF_KEYS;
+                const float key_scale = __ldg(args.block_scales + unlike);
+#pragma unroll
+                for (int j = 0; j < HALF_KEYS; ++j) {
+                    const uint8_t mark = marks[j];
+                    const float of_key = fabsf(key_scale) * cache4::power_of_two(-8 * cache4::key_steps(mark, key_scale < 0.0f));
+                    s[j] = fmaf(s[j] * fminf(row_scale, of_key), fmaxf(row_scale, of_key), -8.0f * cache4::value_steps(mark, key_scale < 0.0f));
+                }
+                scale_log2 = 1.0f;
             }
             const int key_base = (walk_back ? block1 - i : block0 + i) * KEYS + half * HALF_KEYS;
             if (SHAPED) {
@@ -478,7 +491,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             // HALF: the largest weight in use is 2^7 when its scale is new and never more than 2^15, float16's reach, however large the scores are (so
             // what is taken off a score is rounded up); weights under 2^-21 of the largest are the first that float16 holds with fewer bits
-            mx = HALF ? __fmul_ru(mx, scale_log2) : mx * scale_log2;
+            mx = HALF ? __fmaf_ru(mx, scale_log2, value_exponent) : mx * scale_log2;
             const bool grow = mx > (HALF ? __fadd_rd(m_used, 7.0f + RESCALE_THRESHOLD) : m_used + RESCALE_THRESHOLD) || (m_used == -INFINITY && mx != -INFINITY);
             if (__any_sync(0xffffffffu, grow)) {
                 const float m_new = grow ? (HALF ? __fadd_ru(mx, -7.0f) : mx) : m_used;
@@ -496,10 +509,23 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if constexpr (L::APART) tmem_store16(at, reinterpret_cast<const uint32_t*>(o)); else tmem_store32(at, o);
                     }
                 }
-                l *= corr;
+                if constexpr (HALF) {
+                    // (finite: what a key of few bits of value had gathered may be beyond float32 beside one of many)
+                    if (grow) l *= m_used == -INFINITY ? 0.0f : fast_exp2(fminf((m_used - m_new) + (value_exponent - unit), 120.0f));
+                    if (grow) unit = value_exponent;
+                } else {
+                    l *= corr;
+                }
                 m_used = m_new;
             }
-            const float base = (m_used == -INFINITY) ? 0.0f : m_used;
+            const float base = (m_used == -INFINITY) ? 0.0f : HALF ? __fadd_ru(m_used, -value_exponent) : m_used;
+            float unlike_sum = 0.0f;
+            if (HALF && unlike >= 0) {
+                const uint8_t* marks = args.block_marks + (size_t)unlike * KEYS + half * HALF_KEYS;
+                const bool unlike_keys = __ldg(args.block_scales + unlike) < 0.0f;
+#pragma unroll
+                for (int j = 0; j < HALF_KEYS; ++j) unlike_sum += fast_exp2((s[j] - base) + 8.0f * cache4::value_steps(marks[j], unlike_keys));
+            }
             // p = 2^(s * scale - base), two at a time: packed multiply-add, two exponentials, packed sum, one conversion
             // per pair.  (Making a quarter or half of the pairs by a cubic on the floating-point pipes instead of the
             // special-function unit was measured slower: 168 -> 193 and 221 ms for a 32,768-token prompt.)
@@ -523,18 +549,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
                 }
             }
-            if (HALF && value_part != 1.0f) {                             // rare: scales go in steps of 2^8
-                const __half2 part = __float2half2_rn(value_part);
-#pragma unroll
-                for (int j = 0; j < HALF_KEYS / 2; ++j) {
-                    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&packed[j]), part);
-                    packed[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
             {
                 float a0, a1;
                 unpack2(add2(sum_a, sum_b), a0, a1);
-                l += a0 + a1;
+                if (HALF) l += (unlike >= 0 ? unlike_sum : a0 + a1) * fast_exp2(unit - value_exponent);
+                else l += a0 + a1;
             }
             // P_i goes to buffer i & 1, which the products of block i - 2 must have finished reading.  They have: the
             // issuing thread asked for them before it asked for S_i, its products complete in the order it issues them, and
@@ -550,9 +569,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (!mbar_wait(smem_u32(&pv_done[last & 1]), (uint32_t)((last >> 1) & 1))) expired();
         }
         if (args.sinks && half == 0 && row_ok) {
-            // l is the sum of 2^(score * scale_log2 - m_used); the sink's term in the same units
+            // l is the sum of 2^(score * scale_log2 - m_used), with HALF times 2^unit; the sink's term in the same units
             const int sink_head = kh * args.group + (r - local * args.group);
-            l += exp2f(__ldg(args.sinks + sink_head) * 1.4426950408889634f - (m_used == -INFINITY ? 0.0f : m_used));
+            l += exp2f(__ldg(args.sinks + sink_head) * 1.4426950408889634f - (m_used == -INFINITY ? 0.0f : HALF ? m_used - unit : m_used));
         }
         if (SPLIT == 2) {               // the row sum is the two threads' sums together (both rescaled to the same maximum)
             pair_max[n_blocks & 1][half][r] = l;
@@ -561,7 +580,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (ok) {
             fence_after_sync();
-            const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * value_scale;
+            const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * (HALF ? cache4::power_of_two((int)unit) : 1.0f);
             const int token = seq_begin + tok0 + local, head = kh * args.group + (r - local * args.group);
             if constexpr (MAPS) {
                 float* dst = args.maps + (((size_t)(blockIdx.x & 1) * args.n_tokens + token) * args.heads + head) * VD;

@@ -277,9 +277,9 @@ rope_append_4bit_kernel(const float* __restrict__ qkv, int splits, size_t split_
 // those: block w of sequence b goes to place b * span + w - (its first block that is seen), and table_tmp names the places (-1: not
 // seen, or outside the pool).  Tokens behind the sequence's end become zeros.  Bound by the 16 bits a number that it writes.
 // grid = (2 * span, kv_heads, sequences): keys and values are CTAs of their own.
-// HALF: float16 numbers instead, each times a power of two of its block and head, whose inverse goes to scales [keys or values][places][kv_heads]
-// (a bfloat16 number would be m + s n rounded once more, to 8 bits; these have 11).  A group of values that is not a number becomes zeros, so that a
-// product with a weight of zero is zero: the block's scale is then negative, and marks [places][kv_heads][64] names such groups of every token.
+// HALF: float16 numbers instead, each times a power of two of its block and head, or of its token where a block's tokens are unlike, whose inverse goes to scales
+// [keys or values][places][kv_heads] and marks [places][kv_heads][64] (a bfloat16 number would be m + s n rounded once more, to 8 bits; these have 11).  A
+// group of values that is not a number becomes zeros, so that a product with a weight of zero is zero, and is marked.  See cache_4bit.cuh.
 template <bool HALF>
 __device__ __forceinline__ uint32_t two_numbers(float a, float b) {
     if constexpr (HALF) {
@@ -297,7 +297,9 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
                    int pool_blocks, const int* __restrict__ cu, const int* __restrict__ len_before, int kv_heads, int window, int span,
                    uint16_t* __restrict__ keys, uint16_t* __restrict__ values, float* __restrict__ scales, uint8_t* __restrict__ marks, int* __restrict__ table_tmp, unsigned* status) {
     constexpr int G = D / 32;
-    __shared__ float most[8];
+    __shared__ float most[2][8], group_most[2][TT_BLOCK_TOKENS * G];
+    __shared__ uint8_t steps_of[TT_BLOCK_TOKENS];
+    __shared__ unsigned spread_sh;
     tt_pdl_wait();
     tt_pdl_launch_dependents();
     const int b = blockIdx.z, kh = blockIdx.y, place = blockIdx.x >> 1;
@@ -326,38 +328,62 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
     const __nv_bfloat16* tops = reinterpret_cast<const __nv_bfloat16*>(words + code_bytes(D) / 4);            // of values
     const __nv_bfloat16* least = tops + TT_BLOCK_TOKENS * G;
     float down = 1.0f;
+    int exponent = 0, most_steps = 15;
+    bool unlike = false;                                               // tokens have steps of their own
+    auto down_of = [&](int token) { return HALF && unlike ? cache4::power_of_two(8 * min((int)steps_of[token], most_steps) - exponent) : down; };
     if constexpr (HALF) {
-        // the largest number of the block: a thread a group of a token
-        float mine = 0.0f;
+        // the largest number of the block and of each token: a thread a group of a token.  The marks need the keys' and the values'; the values' CTA writes them.
+        const int sides = of_keys ? 1 : 2;
+        float mine[2] = {0.0f, 0.0f};
         bool bad = false;
-        const int token = threadIdx.x / G, g = threadIdx.x % G;
-        if (threadIdx.x < TT_BLOCK_TOKENS * G && token < left) {
-            float s, m;
-            if (of_keys) {
-                const uint32_t pair = __ldg(pairs + threadIdx.x);
-                s = __uint_as_float(pair << 16);
-                m = __uint_as_float(pair & 0xffff0000u);
-            } else {
-                s = __bfloat162float(tops[threadIdx.x]);
-                m = __bfloat162float(least[g * TT_BLOCK_TOKENS + token]);
+        if (threadIdx.x < TT_BLOCK_TOKENS * G && (int)threadIdx.x / G < left) {
+            const uint32_t pair = __ldg(reinterpret_cast<const uint32_t*>(k_pool + from + code_bytes(D)) + threadIdx.x);
+            const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
+            if (s == s) mine[0] = fmaxf(fabsf(m), fabsf(fmaf(15.0f, s, m)));
+            if (!of_keys) {
+                const float vs = __bfloat162float(tops[threadIdx.x]), vm = __bfloat162float(least[threadIdx.x % G * TT_BLOCK_TOKENS + threadIdx.x / G]);
+                bad = vs != vs;
+                if (!bad) mine[1] = fmaxf(fabsf(vm), fabsf(fmaf(15.0f, vs, vm)));
             }
-            bad = s != s;
-            if (!bad) mine = fmaxf(fabsf(m), fabsf(fmaf(15.0f, s, m)));
         }
-        const uint32_t warp_most = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
-        if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = __uint_as_float(warp_most);
-        const bool any_bad = __syncthreads_or(bad) && !of_keys;
-        float largest = most[0];
+        for (int k = 0; k < sides; ++k) {
+            const uint32_t warp_most = __reduce_max_sync(0xffffffffu, __float_as_uint(mine[k]));
+            if ((threadIdx.x & 31) == 0) most[k][threadIdx.x >> 5] = __uint_as_float(warp_most);
+            if (threadIdx.x < TT_BLOCK_TOKENS * G) group_most[k][threadIdx.x] = mine[k];
+        }
+        if (threadIdx.x == 0) spread_sh = 0u;
+        const bool any_bad = __syncthreads_or(bad);
+        int steps[2] = {0, 0};
+        for (int k = 0; k < sides; ++k) {
+            float largest = most[k][0];
 #pragma unroll
-        for (int k = 1; k < 8; ++k) largest = fmaxf(largest, most[k]);
-        const int e = cache4::half_exponent(largest);
-        down = cache4::power_of_two(-e);
+            for (int w = 1; w < 8; ++w) largest = fmaxf(largest, most[k][w]);
+            exponent = cache4::half_exponent(largest);                 // its own kind's at last
+            if (threadIdx.x < TT_BLOCK_TOKENS) {
+                float token_most = 0.0f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) token_most = fmaxf(token_most, group_most[k][threadIdx.x * G + g]);
+                if (token_most > 0.0f) steps[k] = (exponent - cache4::half_exponent(token_most)) >> 3;
+                steps_of[threadIdx.x] = (uint8_t)steps[k];
+                if (steps[k] > 1) atomicOr(&spread_sh, 1u << k);       // more than a step between two tokens (a token of zeros goes with any)
+            }
+        }
+        __syncthreads();
+        const unsigned spread = spread_sh;
+        steps[0] = spread & 1u ? min(steps[0], 15) : 0;
+        most_steps = !of_keys && spread & 1u ? 14 : 15;
+        steps[1] = spread & 2u ? min(steps[1], most_steps) : 0;
+        unlike = spread >> (sides - 1) & 1u;
+        down = cache4::power_of_two(-exponent);
         const size_t slot = ((size_t)b * span + place) * kv_heads + kh;
-        if (threadIdx.x == 0) scales[(of_keys ? 0 : (size_t)gridDim.z * span * kv_heads) + slot] = any_bad ? -cache4::power_of_two(e) : cache4::power_of_two(e);
-        if (any_bad && threadIdx.x < TT_BLOCK_TOKENS) {
+        const bool flagged = of_keys ? unlike : any_bad || unlike;
+        if (threadIdx.x == 0) scales[(of_keys ? 0 : (size_t)gridDim.z * span * kv_heads) + slot] = flagged ? -cache4::power_of_two(exponent) : cache4::power_of_two(exponent);
+        if (!of_keys && threadIdx.x < TT_BLOCK_TOKENS && (flagged || (spread & 1u))) {
             unsigned mask = 0;
-            for (int k = 0; k < G; ++k) mask |= (unsigned)(threadIdx.x < left && tops[threadIdx.x * G + k] != tops[threadIdx.x * G + k]) << k;
-            marks[slot * TT_BLOCK_TOKENS + threadIdx.x] = (uint8_t)mask;
+            for (int k = 0; k < G; ++k) mask |= (unsigned)((int)threadIdx.x < left && tops[threadIdx.x * G + k] != tops[threadIdx.x * G + k]) << k;
+            const unsigned mark = !(spread & 1u) ? (unsigned)steps[1] << 4 | mask
+                                  : mask ? 0xf0u | (steps[0] || steps[1] ? 15u : mask) : (unsigned)(steps[1] << 4 | steps[0]);
+            marks[slot * TT_BLOCK_TOKENS + threadIdx.x] = (uint8_t)mark;
         }
     }
     if (of_keys) {
@@ -366,7 +392,7 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
             const int i = k * 256 + threadIdx.x;
             const int c = i & 3, g = (i >> 2) % G, token = (i >> 2) / G;       // eight neighbouring numbers
             const uint32_t word = __ldg(words + (token * 4 + c) * G + g), pair = __ldg(pairs + token * G + g);
-            const float s = __uint_as_float(pair << 16) * down, m = __uint_as_float(pair & 0xffff0000u) * down;
+            const float times = down_of(token), s = __uint_as_float(pair << 16) * times, m = __uint_as_float(pair & 0xffff0000u) * times;
             uint32_t out[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -383,15 +409,18 @@ expand_4bit_kernel(const uint8_t* __restrict__ k_pool, const uint8_t* __restrict
         const uint32_t word = __ldg(words + (((a * G + g) * 8 + r) * 4 + c) * 2 + jj);
         const uint2 low = __ldg(reinterpret_cast<const uint2*>(least + g * TT_BLOCK_TOKENS + token));
         const float m[4] = {__uint_as_float(low.x << 16), __uint_as_float(low.x & 0xffff0000u), __uint_as_float(low.y << 16), __uint_as_float(low.y & 0xffff0000u)};
-        float s[4];
+        float s[4], times[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] = __bfloat162float(tops[(token + k) * G + g]) * down;
+        for (int k = 0; k < 4; ++k) {
+            times[k] = down_of(token + k);
+            s[k] = __bfloat162float(tops[(token + k) * G + g]) * times[k];
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float x[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                x[k] = token + k < left && (!HALF || s[k] == s[k]) ? fmaf(s[k], (float)((word >> (4 * (2 * (k >> 1) + e) + 16 * (k & 1))) & 15u), m[k] * down) : 0.0f;
+                x[k] = token + k < left && (!HALF || s[k] == s[k]) ? fmaf(s[k], (float)((word >> (4 * (2 * (k >> 1) + e) + 16 * (k & 1))) & 15u), m[k] * times[k]) : 0.0f;
             const uint2 v = make_uint2(two_numbers<HALF>(x[0], x[1]), two_numbers<HALF>(x[2], x[3]));
             *reinterpret_cast<uint2*>(values + to + (size_t)(32 * g + 16 * jj + 8 * e + r) * TT_BLOCK_TOKENS + token) = v;
         }

@@ -35,6 +35,17 @@ __device__ __forceinline__ int half_exponent(float largest) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Float16 blocks (cache_4bit.cu makes them, attention_tcgen05.cu reads them) have a power of two a block and head, for keys and for values.  Where a
+// token's largest number is of another step of 2^8 and not of the next one, the block's tokens have powers of their own: 2^-8 of the block's for each of
+// the token's steps, so that a large token takes no bits from its neighbours.  A mark a token says how many:
+//   keys' scale positive: the low four bits are the groups of 32 values that are not numbers (held as zeros), the high four the values' steps; looked at
+//     where the values' scale is negative;
+//   keys' scale negative: the low four bits are the keys' steps, the high four the values', up to 14; 15 there: the token has no steps, and the low bits are its
+//     groups that are not numbers, all four if it had steps (whoever sees such a token gets NaN in its whole head).
+__device__ __forceinline__ int key_steps(uint8_t mark, bool unlike_keys) { return unlike_keys && mark < 0xf0 ? mark & 15 : 0; }
+__device__ __forceinline__ int value_steps(uint8_t mark, bool unlike_keys) { return unlike_keys && mark >= 0xf0 ? 0 : mark >> 4; }
+__device__ __forceinline__ unsigned marked_groups(uint8_t mark, bool unlike_keys) { return unlike_keys && mark < 0xf0 ? 0u : mark & 15u; }
+
 inline bool takes(int heads, int kv_heads, int head_dim) {
     return kv_heads > 0 && kv_heads <= 65535 && heads % kv_heads == 0 && heads / kv_heads >= 1 && heads / kv_heads <= 16 &&
            (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128);

@@ -1339,8 +1339,11 @@ def expand_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
     are zero, and places that it does not fill stay as they are.  ``table_tmp`` (int32, like ``table``) names the place of every block, -1 for those not
     seen: with it, ``keys`` and ``values`` are what a plain cache's pools and table would be.  With ``scales`` (float32 ``[2, places, kv_heads]``) and
     ``marks`` (uint8 ``[places, kv_heads, 64]``) ``keys`` and ``values`` are float16 instead, to be multiplied by the power of two of their place and head
-    (``scales[0]`` the keys', ``scales[1]`` the values'): three bits more of every number, for :func:`attention_half`.  Groups of values that are NaN
-    are zeros there, the place's scale is negative, and the token's mark has the group's bit."""
+    (``scales[0]`` the keys', ``scales[1]`` the values', without their signs): three bits more of every number, for :func:`attention_half`.  Where the largest numbers of a place's
+    tokens lie more than 2^8 apart, each token's are kept 2^(8 steps) larger still, and the scale is negative; a negative scale of values may also mean groups that are
+    NaN, which are held as zeros.  ``marks`` then has the steps and groups of every token: with a positive scale of keys the low four bits are the groups that are NaN and the high
+    four the values' steps; with a negative one the low four are the keys' steps and the high four the values', or the high four are 15, the token has no steps and the low four are
+    its NaN groups (15, the whole head, where a token with a NaN group would have had steps)."""
     dtype = torch.bfloat16 if scales is None else torch.float16
     _need(keys, dtype, "expanded keys")
     _need(values, dtype, "expanded values")
