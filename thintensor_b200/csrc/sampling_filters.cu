@@ -728,7 +728,8 @@ extern "C" int tt_sample_filtered(const float* logits, long long ld, int rows, i
                                   const float* top_ps, float top_p, const float* min_ps, float min_p, const float* uniforms, unsigned long long seed,
                                   const int* requests, const int* steps, int* out, cudaStream_t stream) {
     if (rows <= 0) return 0;
-    if (vocab <= 0 || vocab > MAX_CLUSTER * MOST_SLICE || (!uniforms && (!requests || !steps))) return (int)cudaErrorInvalidValue;
+    // one number short of what the slices could hold: 2^19 equal weights of 2^45 come to 2^64
+    if (vocab <= 0 || vocab >= MAX_CLUSTER * MOST_SLICE || (!uniforms && (!requests || !steps))) return (int)cudaErrorInvalidValue;
     int sms = 0;
     cudaError_t code = tt_sm_count(&sms);
     if (code != cudaSuccess) return (int)code;

@@ -2009,7 +2009,7 @@ def sample_rows(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
               _ptr(request), _ptr(step), _ptr(out), _stream()), "sample_rows")
 
 
-SAMPLE_FILTERED_VOCAB = 8 * 65536
+SAMPLE_FILTERED_VOCAB = 8 * 65536 - 1                       # the sum of so many weights of up to 2^45 units fits 64 bits
 
 
 def _row_setting(value, dtype: torch.dtype, rows: int, name: str, low: float | None = None, high: float | None = None) -> tuple:
