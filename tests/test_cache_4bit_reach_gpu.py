@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import plain_cache_4bit as plain
-from test_cache_4bit_gpu import Step, queries, run_attention
+from test_cache_4bit_gpu import Step, close_to, queries, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -102,6 +102,16 @@ def test_a_value_of_little_weight(dim, group, token, factor, splits):
     enlarge(step, "v", 0, token, factor)
     q = queries(step, 2 * group).abs()
     close_to_own(run_attention(step, q, 2 * group, splits=splits, one=True), step, q, 2 * group)
+
+
+@pytest.mark.parametrize("splits", [1, 4, 0])
+def test_sinks_of_minus_infinity_are_none(splits):
+    """Also for rows that see no key in a slice: of several tokens with a window the last ones start behind the first slice."""
+    step = Step([895, 70], [8, 2], 2, 64)
+    q = queries(step, 8)
+    sinks = torch.tensor([-math.inf, 1.0, -math.inf, 0.0, -math.inf, 2.0, -math.inf, -math.inf], device=DEV)
+    for window in (0, 60, 2):
+        close_to(run_attention(step, q, 8, window=window, splits=splits, sinks=sinks), step, q, 8, window=window, sinks=sinks)
 
 
 # ----------------------------------------------------------------------------------------------- prompts over copies

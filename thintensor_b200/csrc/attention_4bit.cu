@@ -727,7 +727,7 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             const float ms = __ldg(sinks + head) * 1.4426950408889634f;
             const float m2 = fmaxf(m, ms);
             const float keep = m == -INFINITY ? 0.0f : exp2f(m - m2);
-            l = fmaf(l, keep, exp2f(ms - m2));
+            l = fmaf(l, keep, ms == -INFINITY ? 0.0f : exp2f(ms - m2));      // (a slice in which the row sees no key has m = -inf, too)
             acc0 *= keep;
             acc1 *= keep;
             m = m2;
