@@ -104,6 +104,20 @@ def test_a_value_of_little_weight(dim, group, token, factor, splits):
     close_to_own(run_attention(step, q, 2 * group, splits=splits, one=True), step, q, 2 * group)
 
 
+@pytest.mark.parametrize("splits", [1, 0])
+def test_a_value_that_is_no_number_counts_however_little_it_weighs(splits):
+    """A weight that is zero in float32 times NaN is NaN wherever the row sees the value: in its last block as in those before it."""
+    for token in (130, 20):
+        step = Step([140], [1], 2, 64)
+        turn_away(step, 0, token, 32.0)
+        step.cache.poison("v", 0, token, 1, 0)
+        step.k_pool, step.v_pool = step.cache.pools()
+        got = run_attention(step, queries(step, 8).abs(), 8, splits=splits, one=True).view(8, 64)
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[4:, :32] = True
+        assert torch.equal(torch.isnan(got), bad)
+
+
 @pytest.mark.parametrize("splits", [1, 4, 0])
 def test_sinks_of_minus_infinity_are_none(splits):
     """Also for rows that see no key in a slice: of several tokens with a window the last ones start behind the first slice."""

@@ -256,8 +256,13 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
                 float& x = s[kt][nq][hi];
                 float& y = s[kt][nq][hi + 1];
                 fma_two(x, y, x, y, st.scale[nq][0], st.scale[nq][1], base[0], base[1]);
-                x = fast_exp2(x);
-                y = fast_exp2(y);
+                if constexpr (MASKED) {                                // a masked key weighs minus zero: told from a weight too small for float32
+                    x = x == -INFINITY ? -0.0f : fast_exp2(x);
+                    y = y == -INFINITY ? -0.0f : fast_exp2(y);
+                } else {
+                    x = fast_exp2(x);
+                    y = fast_exp2(y);
+                }
                 add_two(sum[0], sum[1], x, y);
             }
 #pragma unroll
@@ -278,6 +283,7 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
             st.least[nq][0] *= corr[nq][0]; st.least[nq][1] *= corr[nq][1];
         }
     }
+    auto masked = [](float p) { return __float_as_uint(p) == 0x80000000u; };
     constexpr int SETS = DUP ? (G + 1) / 2 : G;                        // operands of weights: with DUP one holds two groups'
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
@@ -321,8 +327,8 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
             for (int nq = 0; nq < NQ; ++nq) {
                 float p0 = s[kt][nq][0] * s0, p1 = s[kt][nq][1] * s0, p2 = s[kt][nq][2] * s1, p3 = s[kt][nq][3] * s1;
                 if constexpr (MASKED) {                                // a masked value adds nothing, whatever its scale
-                    p0 = s[kt][nq][0] == 0.0f ? 0.0f : p0; p1 = s[kt][nq][1] == 0.0f ? 0.0f : p1;
-                    p2 = s[kt][nq][2] == 0.0f ? 0.0f : p2; p3 = s[kt][nq][3] == 0.0f ? 0.0f : p3;
+                    p0 = masked(s[kt][nq][0]) ? 0.0f : p0; p1 = masked(s[kt][nq][1]) ? 0.0f : p1;
+                    p2 = masked(s[kt][nq][2]) ? 0.0f : p2; p3 = masked(s[kt][nq][3]) ? 0.0f : p3;
                 }
                 b0[nq] = transpose_8x8(pack_f16(p0, p1));
                 b1[nq] = transpose_8x8(pack_f16(p2, p3));
