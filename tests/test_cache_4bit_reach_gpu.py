@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import plain_cache_4bit as plain
-from test_cache_4bit_gpu import Step, close_to, queries, run_attention
+from test_cache_4bit_gpu import Step, close_to, layer, queries, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -251,3 +251,17 @@ def test_prompts_give_the_same_bits_every_time(dim):
     for _ in range(20):
         assert torch.equal(run_prompt(step, q, 32), first)
     assert int(step.status.item()) == 0
+
+
+# ----------------------------------------------------------------------------------------------- the layer's copies
+@pytest.mark.parametrize("options", [dict(), dict(window=100), dict(chunk=64)])
+def test_prompts_of_one_sequence_among_many_without_a_token(options):
+    """A step whose tokens are nearly all one sequence's: the copies have places for all that it sees."""
+    before, new = [700] + [3] * 199, [300] + [0] * 198 + [1]
+    step = Step(before, new, 2, 64)
+    mixer, ctx, cache = layer(step, 8, False, **options)
+    mixer.expands_4bit = lambda ctx, width: True
+    q = queries(step, 8)
+    out = torch.full_like(q, 7.0)
+    mixer.attend(ctx, q, cache, step.table, out)
+    close_to_own(out, step, q, 8, window=mixer.reach, copied=True)

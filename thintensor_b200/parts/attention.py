@@ -341,11 +341,11 @@ class CausalAttention(Mixer):
 
     def span_4bit(self, ctx, width: int) -> int:
         """Blocks that a sequence of the step can see, from the step's shape alone (a replayed step has other lengths): all of
-        its table, or what its new tokens and the window or chunk before them can touch."""
+        its table, or what its new tokens and the window or chunk before them can touch, were they all the step's (the others may bring none)."""
         bound = self.window or self.chunk
         if not bound:
             return width
-        return min(width, (ctx.n_tokens - ctx.sequences + 1 + bound - 1 + 62) // 64 + 1)
+        return min(width, (ctx.n_tokens + bound - 1 + 62) // 64 + 1)
 
     def keys_4bit(self, ctx) -> int:
         """How many keys a token of the step sees at most."""
