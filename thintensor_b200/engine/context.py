@@ -36,7 +36,8 @@ class Workspace:
     asks for more than it holds and otherwise keeps its address, so steps of a shape
     that has run before allocate nothing (a requirement for graph replay).  A buffer that
     has to grow at least doubles, so a run of slightly longer and longer steps moves it
-    (and makes every captured decode step be captured again) only a few times."""
+    (and makes every captured decode step be captured again) only a few times.  ``most``
+    bounds what that adds: a buffer doubles up to so many bytes and then has what is asked for."""
 
     def __init__(self, device: torch.device):
         self.device = device
@@ -45,7 +46,7 @@ class Workspace:
         self.generation = 0  # bumped whenever a buffer moves
         self._zeroed: set[str] = set()                # names handed out by get_zeroed
 
-    def get(self, name: str, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
+    def get(self, name: str, shape: tuple[int, ...], dtype: torch.dtype, most: int | None = None) -> torch.Tensor:
         key = (name, shape, dtype)
         view = self._views.get(key)
         if view is not None:
@@ -56,7 +57,8 @@ class Workspace:
         nbytes = count * torch.empty((), dtype=dtype).element_size()
         buffer = self._buffers.get(name)
         if buffer is None or buffer.numel() < nbytes:
-            grow = max(nbytes, 2 * buffer.numel() if buffer is not None else 0, 256)
+            double = 2 * buffer.numel() if buffer is not None else 0
+            grow = max(nbytes, double if most is None else min(double, most // 256 * 256), 256)
             grow = -(-grow // 256) * 256
             buffer = None                                                    # the old one goes before the new one comes
             self._buffers.pop(name, None)
@@ -113,5 +115,5 @@ class StepContext:
     residual: torch.Tensor | None = None                    # float32 [n_tokens, hidden]: set by an arrangement whose parts may add into the stream themselves
     memo: dict = field(default_factory=dict)                # what a part computed for this step that its other layers can use again
 
-    def scratch(self, name: str, shape: tuple[int, ...], dtype: torch.dtype | None = None) -> torch.Tensor:
-        return self.workspace.get(name, shape, dtype or self.act_dtype)
+    def scratch(self, name: str, shape: tuple[int, ...], dtype: torch.dtype | None = None, most: int | None = None) -> torch.Tensor:
+        return self.workspace.get(name, shape, dtype or self.act_dtype, most)

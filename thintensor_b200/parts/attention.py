@@ -337,7 +337,7 @@ class CausalAttention(Mixer):
         return ctx.workspace.get_zeroed("attention.tickets", (max(ctx.sequences * self.kv_heads, 64),), torch.int32)
 
     # ------------------------------------------------------------------ a cache in 4 bits
-    EXPAND_4BIT_BYTES = 4 << 30     # most scratch memory that the expanded blocks may take
+    EXPAND_4BIT_BYTES = 4 << 30     # most scratch memory that the copies of keys and values may take together
 
     def span_4bit(self, ctx, width: int) -> int:
         """Blocks that a sequence of the step can see, from the step's shape alone (a replayed step has other lengths): all of
@@ -370,8 +370,8 @@ class CausalAttention(Mixer):
         if self.expands_4bit(ctx, width):
             places = ctx.sequences * self.span_4bit(ctx, width)
             named = ctx.scratch("attention.table", tuple(table.shape), torch.int32)
-            keys = ctx.scratch("attention.keys", (places, self.kv_heads, 64, self.head_dim), torch.float16)
-            values = ctx.scratch("attention.values", (places, self.kv_heads, self.head_dim, 64), torch.float16)
+            keys = ctx.scratch("attention.keys", (places, self.kv_heads, 64, self.head_dim), torch.float16, most=self.EXPAND_4BIT_BYTES // 2)
+            values = ctx.scratch("attention.values", (places, self.kv_heads, self.head_dim, 64), torch.float16, most=self.EXPAND_4BIT_BYTES // 2)
             scales = ctx.scratch("attention.scales", (2, places, self.kv_heads), torch.float32)
             marks = ctx.scratch("attention.marks", (places, self.kv_heads, 64), torch.uint8)
             api.expand_4bit(cache.k_pool, cache.v_pool, table, ctx.cu, ctx.len_before, ctx.sequences, self.reach, keys, values, named, ctx.status,
