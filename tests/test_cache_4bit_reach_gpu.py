@@ -253,6 +253,36 @@ def test_prompts_give_the_same_bits_every_time(dim):
     assert int(step.status.item()) == 0
 
 
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 40, 2.0 ** 80, 2.0 ** 110])
+@pytest.mark.parametrize("empty", [(0, 64), (64, 128), (30, 50), (128, 199)])
+@pytest.mark.parametrize("copied", [True])
+def test_values_of_zero_beside_large_ones(factor, empty, copied):
+    """What weighs as much as anything and adds nothing counts among the weights, before the large values and after them."""
+    step = Step([200], [6], 2, 64, value_scale=factor)
+    _, s, m = step.cache.v_parts
+    for token in range(*empty):
+        block, at = int(step.cache.table[0, token // 64]), token % 64
+        s[block, :, at], m[block, :, at] = 0.0, 0.0
+    rewrite(step, "v")
+    q = queries(step, 8)
+    for splits in (None,) if copied else (1, 3, 0):
+        close_to_own(run_prompt(step, q, 8) if copied else run_attention(step, q, 8, splits=splits), step, q, 8, copied=copied)
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 90, 2.0 ** -90])
+@pytest.mark.parametrize("copied", [True])
+def test_values_that_are_all_alike(size, copied):
+    """Groups whose scale is zero: their least values are all there is."""
+    step = Step([200], [6], 2, 64)
+    n, s, m = step.cache.v_parts
+    n.zero_(), s.zero_(), m.fill_(size)
+    m[..., 1] = -size
+    rewrite(step, "v")
+    q = queries(step, 8)
+    for splits in (None,) if copied else (1, 3, 0):
+        close_to_own(run_prompt(step, q, 8) if copied else run_attention(step, q, 8, splits=splits), step, q, 8, copied=copied)
+
+
 # ----------------------------------------------------------------------------------------------- the layer's copies
 @pytest.mark.parametrize("options", [dict(), dict(window=100), dict(chunk=64)])
 def test_prompts_of_one_sequence_among_many_without_a_token(options):

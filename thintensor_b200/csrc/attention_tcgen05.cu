@@ -30,7 +30,8 @@
 // 0.0017 with these, which is the rounding of the outputs).  The softmax threads bring their rows of queries to float16 in place, with a power of two
 // a row, before the first product; the weights are float16 too.  A weight carries its values' power of two: the maximum of a row is one of score + that
 // exponent, so the row's unit depends on what it sees and by how much it weighs it, and on nothing else in the tile (with the largest exponent of the tile's
-// blocks as the unit, a value of 2^34 that later tokens alone see left earlier rows no bits).  The sum of the weights without it, l, is kept beside them.
+// blocks as the unit, a value of 2^34 that later tokens alone see left earlier rows no bits).  The sum of the weights without that exponent, l, has a base of its own,
+// and exponentials of its own in blocks whose values are so much smaller than others that their weights hold too little of it.
 //
 // The reference has no counterpart: it feeds prompts token by token through its
 // single-token attention (thinruntime/cli.py:2802-2807, thinruntime/triton_kernels.py:14-109).
@@ -151,7 +152,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __shared__ uint64_t q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2], p_ready[2], pv_done[2];
     __shared__ uint32_t tmem_base_shared;
     __shared__ int tile_info[2];                                  // sequence, tile within the sequence
-    __shared__ float pair_max[2][2][ROWS];
+    __shared__ float pair_max[HALF ? 3 : 2][2][ROWS];
     __shared__ uint64_t q_ready;                                  // HALF: the queries have been converted
     __shared__ uint64_t v_full[KV_STAGES], v_empty[KV_STAGES];    // APART: the values'; kv_full and kv_empty are the keys'
 
@@ -328,7 +329,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int* table_row = args.table + (size_t)b * args.table_width;
         float row_scale = 1.0f, next_key = 1.0f, next_value = 1.0f;
         int this_block = 0, next_block = 0;
-        float unit = 0.0f;                                        // HALF: l is relative to 2^(m_used - unit), O to 2^m_used
+        // HALF: m_used is of scores in a block whose values' exponent is m_exponent, so O is relative to 2^(m_used + m_exponent); l, of this thread's keys, to 2^l_base
+        float m_exponent = 0.0f, l_base = -INFINITY;
+        bool far_apart = false;                                   // the exponents of the tile's values lie more than 56 apart (the same for the whole warp)
         unsigned not_numbers = 0;                                 // groups of 32 numbers of the row's output
         // a block outside the pool is read as block 0 (and flagged) by the thread that loads it
         auto scales_at = [&](int i) {
@@ -341,6 +344,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             next_key = __ldg(args.block_scales + this_block);
             next_value = __ldg(value_scales + this_block);
             next_block = scales_at(1);
+            unsigned greatest = 0u, least = 255u;
+            for (int i = lane; i < n_blocks; i += 32) {
+                const unsigned exponent = (__float_as_uint(__ldg(value_scales + scales_at(i))) >> 23) & 255u;
+                greatest = max(greatest, exponent);
+                least = min(least, exponent);
+            }
+            far_apart = __reduce_max_sync(0xffffffffu, greatest) > __reduce_min_sync(0xffffffffu, least) + 56u;
             // 64 numbers of the row's queries a thread, 16 bytes a time, each thread from another bank
             if (!mbar_wait(smem_u32(&q_full), 0)) expired();
             uint8_t* row = q_smem + half * ROWS * 128 + r * 128;
@@ -404,18 +414,39 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                     for (int j = 0; j < 32; ++j) s[32 * c + j] = tmem_loaded(raw[c][j]);
             }
-            if (HALF && unlike >= 0) {                                // rare: scores in log2 units, and with the tokens' steps below their block's value exponent
-                const uint8_t* marks = args.block_marks + (size_t)unlike * KEYS + half * HALF_KEYS;
-                const float key_scale = __ldg(args.block_scales + unlike);
-#pragma unroll
-                for (int j = 0; j < HALF_KEYS; ++j) {
-                    const uint8_t mark = marks[j];
-                    const float of_key = fabsf(key_scale) * cache4::power_of_two(-8 * cache4::key_steps(mark, key_scale < 0.0f));
-                    s[j] = fmaf(s[j] * fminf(row_scale, of_key), fmaxf(row_scale, of_key), -8.0f * cache4::value_steps(mark, key_scale < 0.0f));
-                }
-                scale_log2 = 1.0f;
-            }
             const int key_base = (walk_back ? block1 - i : block0 + i) * KEYS + half * HALF_KEYS;
+            // Rare: tokens of their own exponents, or values so far apart that their weights hold too little of l, which then takes exponentials of its own.
+            // (All of it here: a branch between the maximum and the exponentials cost every block 12 % at heads of 64.)
+            const bool apart = HALF && (unlike >= 0 || far_apart);
+            if (apart) {
+                const uint8_t* marks = args.block_marks + (size_t)max(unlike, 0) * KEYS + half * HALF_KEYS;
+                float own_scale = scale_log2;
+                bool unlike_keys = false;
+                if (unlike >= 0) {                                    // scores in log2 units, and with the tokens' steps below their block's value exponent
+                    const float key_scale = __ldg(args.block_scales + unlike);
+                    unlike_keys = key_scale < 0.0f;
+#pragma unroll
+                    for (int j = 0; j < HALF_KEYS; ++j) {
+                        const float of_key = fabsf(key_scale) * cache4::power_of_two(-8 * cache4::key_steps(marks[j], unlike_keys));
+                        s[j] = fmaf(s[j] * fminf(row_scale, of_key), fmaxf(row_scale, of_key), -8.0f * cache4::value_steps(marks[j], unlike_keys));
+                    }
+                    scale_log2 = own_scale = 1.0f;
+                }
+                auto score = [&](int j) {
+                    const bool seen = key_base + j <= pos && key_base + j >= first;
+                    return seen ? fmaf(s[j], own_scale, unlike >= 0 ? 8.0f * cache4::value_steps(marks[j], unlike_keys) : 0.0f) : -INFINITY;
+                };
+                float most = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < HALF_KEYS; ++j) most = fmaxf(most, score(j));
+                if (most > l_base + 64.0f) {
+                    l *= fast_exp2(l_base - most);
+                    l_base = most;
+                }
+                const float from = l_base == -INFINITY ? 0.0f : l_base;
+#pragma unroll
+                for (int j = 0; j < HALF_KEYS; ++j) l += fast_exp2(score(j) - from);
+            }
             if (SHAPED) {
                 // Otherwise cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), one exponential and one reciprocal (the
                 // hardware's own tanh is good to 2^-11 of its value, which at a cap of 50 is 0.02 of a score near the cap).
@@ -491,11 +522,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             // HALF: the largest weight in use is 2^7 when its scale is new and never more than 2^15, float16's reach, however large the scores are (so
             // what is taken off a score is rounded up); weights under 2^-21 of the largest are the first that float16 holds with fewer bits
-            mx = HALF ? __fmaf_ru(mx, scale_log2, value_exponent) : mx * scale_log2;
-            const bool grow = mx > (HALF ? __fadd_rd(m_used, 7.0f + RESCALE_THRESHOLD) : m_used + RESCALE_THRESHOLD) || (m_used == -INFINITY && mx != -INFINITY);
+            mx = HALF ? __fmul_ru(mx, scale_log2) : mx * scale_log2;
+            const float m_here = HALF ? __fadd_ru(m_used, m_exponent - value_exponent) : m_used;        // for this block's values
+            const bool grow = mx > (HALF ? __fadd_rd(m_here, 7.0f + RESCALE_THRESHOLD) : m_here + RESCALE_THRESHOLD) || (m_here == -INFINITY && mx != -INFINITY);
             if (__any_sync(0xffffffffu, grow)) {
-                const float m_new = grow ? (HALF ? __fadd_ru(mx, -7.0f) : mx) : m_used;
-                const float corr = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
+                const float m_new = grow ? (HALF ? __fadd_ru(mx, -7.0f) : mx) : m_here;
+                const float corr = (m_here == -INFINITY) ? 0.0f : fast_exp2(m_here - m_new);
                 if (i > 0) {
                     if (ok && !mbar_wait(smem_u32(&pv_done[(i - 1) & 1]), (uint32_t)(((i - 1) >> 1) & 1))) expired();
                     fence_after_sync();
@@ -510,22 +542,21 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                 }
                 if constexpr (HALF) {
-                    // (finite: what a key of few bits of value had gathered may be beyond float32 beside one of many)
-                    if (grow) l *= m_used == -INFINITY ? 0.0f : fast_exp2(fminf((m_used - m_new) + (value_exponent - unit), 120.0f));
-                    if (grow) unit = value_exponent;
+                    if (grow) {
+                        m_used = m_new;
+                        m_exponent = value_exponent;
+                        if (m_new > l_base + RESCALE_THRESHOLD) {     // as long as all values have one exponent l's base moves along
+                            l *= fast_exp2(l_base - m_new);           // (0 at first)
+                            l_base = m_new;
+                        }
+                    }
                 } else {
                     l *= corr;
+                    m_used = m_new;
                 }
-                m_used = m_new;
             }
-            const float base = (m_used == -INFINITY) ? 0.0f : HALF ? __fadd_ru(m_used, -value_exponent) : m_used;
-            float unlike_sum = 0.0f;
-            if (HALF && unlike >= 0) {
-                const uint8_t* marks = args.block_marks + (size_t)unlike * KEYS + half * HALF_KEYS;
-                const bool unlike_keys = __ldg(args.block_scales + unlike) < 0.0f;
-#pragma unroll
-                for (int j = 0; j < HALF_KEYS; ++j) unlike_sum += fast_exp2((s[j] - base) + 8.0f * cache4::value_steps(marks[j], unlike_keys));
-            }
+            float base = (m_used == -INFINITY) ? 0.0f : m_used;
+            if (HALF && m_exponent != value_exponent) base = (m_used == -INFINITY) ? 0.0f : m_here;
             // p = 2^(s * scale - base), two at a time: packed multiply-add, two exponentials, packed sum, one conversion
             // per pair.  (Making a quarter or half of the pairs by a cubic on the floating-point pipes instead of the
             // special-function unit was measured slower: 168 -> 193 and 221 ms for a 32,768-token prompt.)
@@ -552,8 +583,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             {
                 float a0, a1;
                 unpack2(add2(sum_a, sum_b), a0, a1);
-                if (HALF) l += (unlike >= 0 ? unlike_sum : a0 + a1) * fast_exp2(unit - value_exponent);
-                else l += a0 + a1;
+                if (!HALF) l += a0 + a1;
+                else if (!apart) l += (a0 + a1) * fast_exp2(l_base == -INFINITY ? 0.0f : base - l_base);
             }
             // P_i goes to buffer i & 1, which the products of block i - 2 must have finished reading.  They have: the
             // issuing thread asked for them before it asked for S_i, its products complete in the order it issues them, and
@@ -569,18 +600,30 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (!mbar_wait(smem_u32(&pv_done[last & 1]), (uint32_t)((last >> 1) & 1))) expired();
         }
         if (args.sinks && half == 0 && row_ok) {
-            // l is the sum of 2^(score * scale_log2 - m_used), with HALF times 2^unit; the sink's term in the same units
+            // l is the sum of 2^(score * scale_log2 - m_used), or of - l_base; the sink's term in the same units
             const int sink_head = kh * args.group + (r - local * args.group);
-            l += exp2f(__ldg(args.sinks + sink_head) * 1.4426950408889634f - (m_used == -INFINITY ? 0.0f : HALF ? m_used - unit : m_used));
+            l += exp2f(__ldg(args.sinks + sink_head) * 1.4426950408889634f - ((HALF ? l_base : m_used) == -INFINITY ? 0.0f : HALF ? l_base : m_used));
         }
         if (SPLIT == 2) {               // the row sum is the two threads' sums together (both rescaled to the same maximum)
             pair_max[n_blocks & 1][half][r] = l;
+            if constexpr (HALF) pair_max[2][half][r] = l_base;
             pair_barrier();
-            l += pair_max[n_blocks & 1][half ^ 1][r];
+            if constexpr (HALF) {
+                const float other = pair_max[2][half ^ 1][r], both = fmaxf(l_base, other);
+                if (other != l_base) {
+                    l = l * fast_exp2(l_base - both) + pair_max[n_blocks & 1][half ^ 1][r] * fast_exp2(other - both);
+                    l_base = both;
+                } else {
+                    l += pair_max[n_blocks & 1][half ^ 1][r];
+                }
+            } else {
+                l += pair_max[n_blocks & 1][half ^ 1][r];
+            }
         }
         if (ok) {
             fence_after_sync();
-            const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * (HALF ? cache4::power_of_two((int)unit) : 1.0f);
+            float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            if (HALF && m_used != -INFINITY) inv = (inv * exp2f(m_used - l_base)) * cache4::power_of_two((int)m_exponent);
             const int token = seq_begin + tok0 + local, head = kh * args.group + (r - local * args.group);
             if constexpr (MAPS) {
                 float* dst = args.maps + (((size_t)(blockIdx.x & 1) * args.n_tokens + token) * args.heads + head) * VD;
