@@ -255,7 +255,7 @@ def test_prompts_give_the_same_bits_every_time(dim):
 
 @pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 40, 2.0 ** 80, 2.0 ** 110])
 @pytest.mark.parametrize("empty", [(0, 64), (64, 128), (30, 50), (128, 199)])
-@pytest.mark.parametrize("copied", [True])
+@pytest.mark.parametrize("copied", [True, False])
 def test_values_of_zero_beside_large_ones(factor, empty, copied):
     """What weighs as much as anything and adds nothing counts among the weights, before the large values and after them."""
     step = Step([200], [6], 2, 64, value_scale=factor)
@@ -270,7 +270,7 @@ def test_values_of_zero_beside_large_ones(factor, empty, copied):
 
 
 @pytest.mark.parametrize("size", [1.0, 2.0 ** 90, 2.0 ** -90])
-@pytest.mark.parametrize("copied", [True])
+@pytest.mark.parametrize("copied", [True, False])
 def test_values_that_are_all_alike(size, copied):
     """Groups whose scale is zero: their least values are all there is."""
     step = Step([200], [6], 2, 64)

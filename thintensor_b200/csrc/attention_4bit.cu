@@ -13,10 +13,10 @@
 // Queries are float16 after a power of two that brings a row's greatest number to 2^14: exact but for what lies 2^-28 below that.
 // The weights p s' are rounded to float16 (11 bits): with weights in bfloat16 the two terms of out, which are of opposite sign and
 // each several times their sum, were off by 0.4 % of it.  So that float16 holds them whatever the values' size, the running maximum is
-// one of score + E - 14 in log2 units, E the exponent of the largest of the key's value scales (at least -40), and p is relative to it: a row's weights
-// stay below 2^15, its largest is 2^14 or more, and what falls under 2^-14, float16's last full number, is less than 2^-28 of that.  A row's unit so
-// depends on what it sees, and by how much it weighs it, alone (with the largest scale that the warp had met as the unit, a value of 2^34 that later
-// tokens alone see, or of little weight, left the others no bits).  The second term takes p in two bfloat16 parts (16 bits)
+// one of score + E - 14 in log2 units, E the exponent of the largest of the key's value scales and least values (at least -40), and p is relative to it:
+// a row's weights stay below 2^15, and what falls under 2^-14, float16's last full number, is less than 2^-28 of the row's largest p times scale or least
+// value.  A row's unit so depends on what it sees, and by how much it weighs it, alone (with the largest scale that the warp had met as the unit, a value
+// of 2^34 that later tokens alone see, or of little weight, left the others no bits).  The second term takes p in two bfloat16 parts (16 bits)
 // and m' as it is, the second term of S the queries' sums in three.  All sums are float32.
 //
 // Rows of up to four queries (DUP) stand twice in the tile's eight columns, which would otherwise be half empty: the weights of one
@@ -171,10 +171,10 @@ __device__ __forceinline__ void scores_of_block(const Rows4<D, NQ, DUP>& st, con
     }
 }
 
-// E - 14 of two neighbouring tokens as a pair of bfloat16 numbers: E the exponent of a token's largest scale, at least -40 (positive bfloat16 numbers
-// order like their bits; a scale that is not a number counts for nothing here).
+// E - 14 of two neighbouring tokens as a pair of bfloat16 numbers: E the exponent of a token's largest scale or least value, at least -40 (a scale that is
+// not a number counts for nothing here).
 template <int G>
-__device__ __forceinline__ uint32_t exponents_of(const uint8_t* __restrict__ two_tokens) {
+__device__ __forceinline__ uint32_t exponents_of(const uint8_t* __restrict__ two_tokens, const uint8_t* __restrict__ two_mins) {
     uint32_t w[G];                                                     // G scales of the first token, then those of the second
     load_words<G>(two_tokens, w);
     auto larger = [](uint32_t a, uint32_t b) {
@@ -189,6 +189,8 @@ __device__ __forceinline__ uint32_t exponents_of(const uint8_t* __restrict__ two
         const uint32_t a = larger(w[0], w[1]), b = larger(w[2], w[3]);
         most = larger(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
     }
+#pragma unroll
+    for (int g = 0; g < G; ++g) most = larger(most, *reinterpret_cast<const uint32_t*>(two_mins + g * 2 * TT_BLOCK_TOKENS) & 0x7fff7fffu);
     const uint32_t lo = most & 0xffffu, hi = most >> 16;
     const int first = lo <= 0x7f80u ? (int)(lo >> 7) - 127 : -127, second = hi <= 0x7f80u ? (int)(hi >> 7) - 127 : -127;
     return pack_bf16((float)(max(first, -40) - 14), (float)(max(second, -40) - 14));       // whole numbers below 256: exact
@@ -215,7 +217,7 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
                         if (!(key <= st.pos[nq][e] && key >= st.first[nq][e])) s[kt][nq][2 * hi + e] = -INFINITY;
             }
     }
-    const uint32_t exponents = exponents_of<G>(scales + 2 * lane * 2 * G);         // of tokens 2 lane and 2 lane + 1
+    const uint32_t exponents = exponents_of<G>(scales + 2 * lane * 2 * G, mins + 2 * lane * 2);        // of tokens 2 lane and 2 lane + 1
     float most[NQ][2];
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) most[nq][0] = most[nq][1] = -INFINITY;
@@ -267,7 +269,9 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
             }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            st.l_run[nq][e] = st.l_run[nq][e] * corr[nq][e] + sum[e];
+            // (the factor in two parts: keys whose values are zero may have gathered far more than float32's reach beside large values)
+            const float part = fast_exp2(0.5f * (st.m_run[nq][e] - m_new[e]));
+            st.l_run[nq][e] = m_new[e] == -INFINITY ? sum[e] : st.l_run[nq][e] * part * part + sum[e];
             // a key that is not a number has no part in the maximum; what this warp saw must count all the same where others' results join it
             st.m_run[nq][e] = (m_new[e] == -INFINITY && sum[e] != sum[e]) ? 0.0f : m_new[e];
         }
@@ -666,7 +670,8 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
     }
     done += n_mine;
 
-    // the lanes' shares of the row sums together; the codes' unit out, the least values in
+    // the lanes' shares of the row sums together; the codes' unit out, the least values in; and relative to a power of two at which the weights' sum is 1/2 to 1:
+    // what joins then compares by weight alone, not by the values' size as well
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
@@ -675,15 +680,18 @@ attention_4bit_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __rest
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            st.l_run[nq][e] = l;
+            const int up = l > 0.0f && l < INFINITY ? min((int)(__float_as_uint(l) >> 23) - 126, 120) : 0;
+            const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+            st.l_run[nq][e] = l * down;
+            st.m_run[nq][e] += (float)up;
             if constexpr (DUP) st.least[nq][e] += __shfl_xor_sync(0xffffffffu, st.least[nq][e], 2);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const float add = __shfl_sync(0xffffffffu, st.least[nq][e], 4 * g + c);
 #pragma unroll
                 for (int dt = 2 * g; dt < 2 * g + 2; ++dt) {
-                    st.o[dt][nq][e] = fmaf(st.o[dt][nq][e], 1.0f / CODE_UNIT, add);
-                    st.o[dt][nq][2 + e] = fmaf(st.o[dt][nq][2 + e], 0.0625f / CODE_UNIT, add);
+                    st.o[dt][nq][e] = fmaf(st.o[dt][nq][e], 1.0f / CODE_UNIT, add) * down;
+                    st.o[dt][nq][2 + e] = fmaf(st.o[dt][nq][2 + e], 0.0625f / CODE_UNIT, add) * down;
                 }
             }
         }
