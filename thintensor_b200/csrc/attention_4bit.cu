@@ -352,7 +352,7 @@ __device__ __forceinline__ void values_of_block(Rows4<D, NQ, DUP>& st, const uin
 }
 
 // Sixteen warps an SM (eight with two column tiles), as many as registers hold at D = 128: a block is about 1,200 instructions of a warp, whose
-// chains of loads, products and exponentials take it 3,200 cycles alone, and an SM is busy with four warps a scheduler.  Each warp has one
+// chains of loads, products and exponentials take it 3,200 cycles alone, so four warps keep a scheduler busy.  Each warp has one
 // place for a block of keys and one for a block of values, asked for again as soon as it has read them: the keys arrive under the block's
 // softmax and second product, the values under the next block's first.  (Two places each leave room for eight warps: 65 -> 77 us at
 // 64 sequences of up to 4,096 tokens.)  Few CTAs have eight warps, so that a slice is done sooner, many have four.
@@ -876,7 +876,7 @@ cudaError_t launch_attention(const Attention4& a, int sms, cudaStream_t stream) 
         const int ctas = sms * R::CTAS;
         if ((long long)tiles * a.kv_heads * a.table_width >= 1LL << 30 || a.part_rows < 2LL * ctas * tokens_per_tile * group) return cudaErrorInvalidValue;
         // Not ahead of the kernel before it: whatever of that is still resident would leave an SM without room for one CTA of the grid, which
-        // then starts when another one ends and takes as long again (6 of 592 CTAs: 55 -> 87 us).
+        // then starts when another one ends and takes as long again (measured with CTAs of four warps, where 6 of 592 were late: 55 -> 87 us).
         kernel<<<ctas, WARPS * 32, R::SHARED, stream>>>(a.q, a.k_pool, a.v_pool, a.table, a.table_width, a.pool_blocks, a.cu, a.len_before, a.sequences, a.heads,
                                                         a.kv_heads, tokens_per_tile, a.scale_log2, a.window, 0, a.out, a.part_acc, a.part_ml, a.tickets,
                                                         a.status, a.sinks);

@@ -9,9 +9,10 @@
 // an infinite one: token 0.
 //
 // What must not depend on anything but the row: which token it is.  So the weights are formed in float64 (about 1e-14 relative) and
-// summed as whole numbers of 2^-45: sums of those are exact, whatever their order, and only a random number within 2^-27 / vocabulary or so of a
-// border could tell them from exact real arithmetic.  A float32 sum over 100,000 tokens is off by more than a rare token's
-// whole weight.
+// summed as whole numbers of 2^-45: sums of those are exact, whatever their order.  Against exact real arithmetic a sum is off by the weights' rounding
+// to whole numbers, 2^-46 of the largest weight each and so vocabulary * 2^-46 of it at most (2^-29 at 128,256; what lies below 2^-46 of the largest
+// counts nothing), and only a random number, or a share, that close to a border could tell.  A float32 sum over 100,000 tokens is off by more than a rare
+// token's whole weight.
 //
 // A row is read once, by a cluster of up to 8 CTAs that keep their slices of it in shared memory and talk over distributed shared
 // memory.  One row of 128,256 takes 11 us for a nucleus of few tokens, 13 us with top-k and 25 us for a nucleus of tens of thousands, of which the
