@@ -42,7 +42,7 @@ def turn_away(step, b, token, size):
     rewrite(step, "k")
 
 
-def close_to_own(got, step, q, heads, window=0, copied=False):
+def close_to_own(got, step, q, heads, window=0, copied=False, sinks=None):
     """Every row by what it sees itself.  A score is off by `moved` of the magnitudes that it is added up from, its weight by twice that of itself (the maximum moves
     as well), and so every key counts by its own weight in the output's sum and in the sum of weights.
 
@@ -61,7 +61,10 @@ def close_to_own(got, step, q, heads, window=0, copied=False):
             k_size, v_size = wide(ks) * kn + wide(km).abs(), wide(vs) * vn + wide(vm).abs()
             for j in range(count):
                 seen, row = slice(plain.first_key(have + j, window), have + j + 1), rows[at + j, h]
-                p = torch.softmax((k[seen] @ row) * scale, 0)
+                z = (k[seen] @ row) * scale
+                if sinks is not None:
+                    z = torch.cat((z, sinks[h].double().cpu()[None]))
+                p = torch.softmax(z, 0)[:z.numel() - (sinks is not None)]
                 want, weight = p @ v[seen], p @ v_size[seen]
                 reach = (k_size[seen] @ row.abs()) * scale
                 if copied:
@@ -141,13 +144,13 @@ def copies(step, window=0):
     return keys, values, scales, marks, named
 
 
-def run_prompt(step, q, heads, window=0):
+def run_prompt(step, q, heads, window=0, sinks=None):
     from thintensor_b200.kernels import api
 
     keys, values, scales, marks, named = copies(step, window)
     out = torch.full_like(q, 7.0)
     api.attention_half(q, keys, values, scales, marks, n_tokens=q.shape[0], heads=heads, kv_heads=step.kv, head_dim=step.dim, scale=step.dim ** -0.5, window=window,
-                       out=out, **(step.common() | dict(table=named)))
+                       out=out, sinks=sinks, **(step.common() | dict(table=named)))
     return out
 
 
@@ -281,6 +284,35 @@ def test_values_that_are_all_alike(size, copied):
     q = queries(step, 8)
     for splits in (None,) if copied else (1, 3, 0):
         close_to_own(run_prompt(step, q, 8) if copied else run_attention(step, q, 8, splits=splits), step, q, 8, copied=copied)
+
+
+@pytest.mark.parametrize("window", [40, 100, -64])
+@pytest.mark.parametrize("token", [130, 150, 170, 185])                 # before the windows of some rows or of all, and behind some
+@pytest.mark.parametrize("names", ["v", "k", "kv"])
+@pytest.mark.parametrize("copied", [True, False])
+def test_windows_and_what_lies_before_them(window, token, names, copied):
+    step = Step([170, 30], [40, 9], 2, 64, seed=token)
+    for name in names:
+        enlarge(step, name, 0, token, 2.0 ** 34)
+    q = queries(step, 8)
+    for splits in (None,) if copied else (1, 2, 0):
+        got = run_prompt(step, q, 8, window=window) if copied else run_attention(step, q, 8, window=window, splits=splits)
+        close_to_own(got, step, q, 8, window=window, copied=copied)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 90])
+@pytest.mark.parametrize("copied", [True, False])
+def test_sinks_beside_values_of_unlike_sizes(dim, factor, copied):
+    """The sink joins the weights in their own units: in tiles of unlike blocks, of unlike tokens, and where no key weighs anything beside it."""
+    step = Step([150, 30], [30, 9], 2, dim)
+    for token in (20, 65, 175):
+        enlarge(step, "v", 0, token, factor)
+    sinks = torch.tensor([0.0, 5.0, -3.0, 40.0, -40.0, 1.0, -math.inf, 0.5], device=DEV)
+    q = queries(step, 8)
+    for splits in (None,) if copied else (1, 2, 0):
+        got = run_prompt(step, q, 8, sinks=sinks) if copied else run_attention(step, q, 8, splits=splits, sinks=sinks)
+        close_to_own(got, step, q, 8, copied=copied, sinks=sinks)
 
 
 # ----------------------------------------------------------------------------------------------- the layer's copies
